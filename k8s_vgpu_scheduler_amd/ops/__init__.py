@@ -65,6 +65,12 @@ def lib():
         L.mivgpu_stream_read.argtypes = [vp, ctypes.c_longlong, vp, i, vp]
         L.mivgpu_skinny_plan.argtypes = [i, i, i, i, ip, ip, ip, lp, ip, ip]
         L.mivgpu_decode_chain.argtypes = [ctypes.POINTER(ChainGemm), i, vp, vp]
+        ll = ctypes.c_longlong
+        L.mivgpu_page_plan.argtypes = [vp] * 10 + [i] * 4 + [vp]
+        L.mivgpu_page_commit.argtypes = [vp] * 7 + [i] * 3 + [vp]
+        L.mivgpu_paged_qk_norm_rope_kv.argtypes = [vp, ll] + [vp] * 10 + [i] * 5 + [f, vp]
+        L.mivgpu_paged_attention.argtypes = [vp] * 9 + [i] * 7 + [f, vp]
+        L.mivgpu_sample.argtypes = [vp, ll, i, i] + [vp] * 7 + [vp]
         for fn in ("mivgpu_rmsnorm", "mivgpu_add_rmsnorm", "mivgpu_qk_norm_rope_kv",
                    "mivgpu_decode_attention", "mivgpu_silu_mul", "mivgpu_ops_attn_split",
                    "mivgpu_hwid_probe", "mivgpu_pack_weight", "mivgpu_skinny_gemm",
@@ -73,7 +79,8 @@ def lib():
                    "mivgpu_ops_kv_packed", "mivgpu_decode_attention_fused", "mivgpu_skinny_gemm_norm",
                    "mivgpu_prefill_qk_norm_rope_kv", "mivgpu_prefill_attention", "mivgpu_unpack_weight",
                    "mivgpu_decode_chain", "mivgpu_chain_counter_words", "mivgpu_chain_err_word",
-                   "mivgpu_prefill_gemm"):
+                   "mivgpu_prefill_gemm", "mivgpu_page_plan", "mivgpu_page_commit",
+                   "mivgpu_paged_qk_norm_rope_kv", "mivgpu_paged_attention", "mivgpu_sample"):
             getattr(L, fn).restype = ctypes.c_int
         _lib = L
     return _lib
@@ -776,3 +783,10 @@ class DecodeChain:
 
     def gave_up(self) -> bool:
         return int(self.ctr[chain_err_word()].item()) != 0
+
+
+# --------------------------------------- batched serving on 8-bit pages --
+from k8s_vgpu_scheduler_amd.ops.paged import (  # noqa: E402
+    PAGE, PagedKV, PagePlan, PagePool, page_commit, page_plan, paged_attention, paged_attention_workspace,
+    paged_kv_cache, paged_qk_norm_rope_kv, rope_turns)
+from k8s_vgpu_scheduler_amd.ops.sampling import sample, sample_workspace  # noqa: E402

@@ -1,0 +1,52 @@
+"""Sampling a token for each row of logits (csrc/ops/sample.hip): the sampled sibling of ``decode_tail``'s argmax."""
+
+from __future__ import annotations
+
+import torch
+
+from k8s_vgpu_scheduler_amd import ops
+from k8s_vgpu_scheduler_amd.ops.paged import _launch, _on, _ptr
+
+MAX_VOCAB = 128 * 32768      # csrc/ops/sample.hip CARRIES * CHUNK
+
+
+def sample_workspace(rows: int, vocab: int, device="cuda") -> torch.Tensor:
+    """Workspace of ``sample`` for up to ``rows`` rows of ``vocab`` logits.  Every call leaves it ready for the next;
+    calls that may run at once need one each."""
+    return torch.zeros(0, dtype=torch.int64, device=device)
+
+
+def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None,
+           top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
+           tokens: torch.Tensor | None = None, probs: torch.Tensor | None = None, work: torch.Tensor | None = None):
+    """One token a row -> (tokens int64 [B], probs fp32 [B]: its probability among the kept).
+
+    logits bf16 [B, V] (unit column stride), uniform fp32 [B] in [0, 1), and for each row, or None for off:
+    temperature fp32 (1; at or below 0: the first maximum), top_k int32 (at or below 0: off), top_p fp32 (from 1:
+    off), min_p fp32.  In the order of larger logits (equal ones: lower index), with weights exp((l - max) / T):
+    the first top_k, of these the smallest prefix that has top_p of their weight, of these the ones of at least min_p
+    times the largest weight; the answer is the first whose running sum of weights exceeds uniform times their sum.
+    -inf is a masked token; a row of nothing else gives -1 (probability 0).  A NaN counts as the maximum, as in
+    ``decode_tail`` (probability NaN).  ``work`` from ``sample_workspace``."""
+    if logits.dim() != 2:
+        raise ValueError(f"sample: logits must be [B, V], got {tuple(logits.shape)}")
+    B, V = logits.shape
+    dev = logits.device
+    if logits.dtype != torch.bfloat16 or B < 1 or not 0 < V <= MAX_VOCAB or (V > 1 and logits.stride(1) != 1) \
+            or (B > 1 and logits.stride(0) < V):
+        raise ValueError(f"sample: logits must be bf16 [B, V <= {MAX_VOCAB}] with unit column stride, got "
+                         f"{tuple(logits.shape)} {logits.dtype} strides {logits.stride()}")
+    if tokens is None:
+        tokens = torch.empty(B, dtype=torch.int64, device=dev)
+    if probs is None:
+        probs = torch.empty(B, dtype=torch.float32, device=dev)
+    f32 = torch.float32
+    rows = dict(uniform=(uniform, f32), temperature=(temperature, f32), top_k=(top_k, torch.int32), top_p=(top_p, f32),
+                min_p=(min_p, f32), tokens=(tokens, torch.int64), probs=(probs, f32))
+    _on(dev, "sample", **rows, work=(work, torch.int64))
+    for what, (t, _) in rows.items():
+        if t is not None and tuple(t.shape) != (B,):
+            raise ValueError(f"sample: {what} must have one value a row ({B}), got {tuple(t.shape)}")
+    _launch(dev, "sample", ops.lib().mivgpu_sample, _ptr(logits), logits.stride(0) if B > 1 else V, V, B, _ptr(uniform),
+            _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(tokens), _ptr(probs))
+    return tokens, probs
