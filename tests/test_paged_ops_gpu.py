@@ -1,0 +1,599 @@
+"""The paged 8-bit serving operators on the GPU against plain 64-bit implementations (tests/paged_oracle.py)."""
+
+import math
+
+import numpy as np
+import paged_oracle as oracle
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+PAGE, THETA, EPS = 64, 1e6, 1e-6
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from k8s_vgpu_scheduler_amd import ops as o
+    from k8s_vgpu_scheduler_amd.utils import build
+
+    build.build_ops()
+    o.require_native()
+    return o
+
+
+def dev(x, dtype=torch.int32):
+    return torch.as_tensor(np.ascontiguousarray(x)).to(dtype).cuda()
+
+
+def host(t):
+    return t.cpu().numpy()
+
+
+# ------------------------------------------------------------------- plan --
+def pool_state(lengths, width, spare, seed):
+    """A table with distinct pages for `lengths`, and a ring with `spare` free ones behind."""
+    r = np.random.RandomState(seed)
+    have = -(-np.asarray(lengths) // PAGE)
+    num = int(have.sum()) + spare + 2
+    ids = r.permutation(num)
+    table = np.full((len(lengths), width), -7)
+    at = 0
+    for b, h in enumerate(have):
+        table[b, :h] = ids[at:at + h]
+        at += h
+    head = int(r.randint(num))
+    ring = np.zeros(num, np.int64)
+    ring[(head + np.arange(num - at)) % num] = ids[at:]
+    return table, ring, [head, spare]
+
+
+PLANS = {
+    "one token": ([1], [0], 4, 1, 9),
+    "nothing new": ([0, 0], [3, 0], 2, 0, 5),
+    "no tokens, no rows": ([0], [0], 1, 0, 0),
+    "page border": ([1, 1, 1, 64, 65], [63, 64, 65, 0, 0], 4, 20, 132),
+    "padded rows": ([3, 0, 2], [10, 5, 0], 3, 9, 40),
+    "out of pages": ([70, 65, 1, 200], [10, 0, 3, 0], 8, 3, 400),
+    "refused, then one that needs none": ([65, 130, 1], [0, 0, 3], 8, 2, 400),
+    "wider than the table": ([200, 64], [0, 64], 2, 9, 400),
+    "more tokens than rows": ([50, 60, 5], [0, 0, 0], 4, 9, 112),
+    "negative counts as none": ([-5, 3], [7, 0], 2, 4, 3),
+    "ring empty": ([1, 1], [64, 3], 4, 0, 2),
+}
+
+
+@pytest.mark.parametrize("case", PLANS, ids=list(PLANS))
+def test_plan(ops, case):
+    new, old, width, spare, n = PLANS[case]
+    check_plan(ops, new, old, width, spare, n, seed=3)
+
+
+@pytest.mark.parametrize("rows,tokens,seed", [(32, 1, 1), (256, 40, 2), (1000, 3, 3), (1024, 9, 4), (5, 9000, 5)])
+def test_plan_many(ops, rows, tokens, seed):
+    r = np.random.RandomState(seed)
+    new, old = r.randint(0, tokens + 1, rows), r.randint(0, 5000, rows)
+    need = int((-(-(old + new) // PAGE) - -(-old // PAGE)).sum())
+    for spare in (need, max(0, need - 3)):
+        check_plan(ops, new, old, -(-int((old + new).max()) // PAGE), spare, int(new.sum()) + 7, seed)
+
+
+def check_plan(ops, new, old, width, spare, n, seed):
+    table, free, ring = pool_state(old, width, spare, seed)
+    t, f, rg, ln, nw = dev(table), dev(free), dev(ring), dev(old), dev(new)
+    want = oracle.plan(new, old, table, free, ring, n)
+    for _ in range(2):                                   # planning again changes nothing
+        got = ops.page_plan(nw, ln, t, f, rg, n)
+        for name in ("cu_q", "kv_lens", "taken", "positions", "slots"):
+            assert np.array_equal(host(getattr(got, name)), want[name]), name
+        assert np.array_equal(host(t), want["table"])
+        assert np.array_equal(host(f), free) and np.array_equal(host(rg), ring) and np.array_equal(host(ln), old)
+
+
+def test_plan_into_given_buffers(ops):
+    pool = ops.PagePool(40, 3, 6)
+    new = dev([5, 70, 0])
+    a = pool.plan(new, 80)
+    b = ops.PagePlan(*(torch.full_like(x, 99) for x in a))
+    assert pool.plan(new, 80, out=b) is b
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("num", [30, 14])
+def test_pool_serves_requests_to_the_end(ops, num):
+    """Requests come, grow and finish: no page is lost, doubled or shared, and every slot of a request keeps its page."""
+    r = np.random.RandomState(0)
+    B, W = 9, 7
+    pool = ops.PagePool(num, B, W)
+    lengths = np.zeros(B, np.int64)
+    table = host(pool.table).copy()
+    free, ring = host(pool.free).copy(), host(pool.ring).copy()
+    refused = 0
+    for step in range(60):
+        new = np.where(r.rand(B) < 0.7, np.where(lengths == 0, r.randint(1, 200, B), r.randint(0, 3, B)), 0)
+        n = int(new.sum())
+        want = oracle.plan(new, lengths, table, free, ring, n)
+        plan = pool.plan(dev(new), n)
+        assert np.array_equal(host(plan.slots), want["slots"]) and np.array_equal(host(plan.taken), want["taken"])
+        ok = want["taken"] >= 0
+        refused += int((~ok).sum())
+        finished = (r.rand(B) < 0.15) | (lengths + new > 300)
+        pool.commit(plan, torch.as_tensor(finished).cuda())
+        # the same by hand
+        table = want["table"]
+        ring[0] = (ring[0] + want["taken"][ok].sum()) % num
+        ring[1] -= want["taken"][ok].sum()
+        lengths = np.where(ok, want["kv_lens"], lengths)
+        for b in np.flatnonzero(finished):
+            for j in range(-(-lengths[b] // PAGE)):
+                free[(ring[0] + ring[1]) % num] = table[b, j]
+                ring[1] += 1
+            lengths[b] = 0
+        assert np.array_equal(host(pool.lengths), lengths) and np.array_equal(host(pool.ring), ring)
+        assert np.array_equal(host(pool.free)[(ring[0] + np.arange(ring[1])) % num], free[(ring[0] + np.arange(ring[1])) % num])
+        held = [table[b, j] for b in range(B) for j in range(-(-lengths[b] // PAGE))]
+        left = free[(ring[0] + np.arange(ring[1])) % num].tolist()
+        assert sorted(held + left) == list(range(num))
+    assert num > 14 or refused > 0                      # the small pool runs out at times
+
+
+def test_commit_twice_takes_once(ops):
+    pool = ops.PagePool(10, 2, 4)
+    plan = pool.plan(dev([100, 3]), 103)
+    pool.commit(plan)
+    pool.commit(plan)
+    assert host(pool.lengths).tolist() == [100, 3] and host(pool.ring).tolist() == [3, 7]
+
+
+# ----------------------------------------------------------------- append --
+def layout(old, new, seed, spare=2, pad=0):
+    """positions, slots (padding: -1), a table and the pages of a pool that holds the step."""
+    r = np.random.RandomState(seed)
+    old, new = np.asarray(old), np.asarray(new)
+    have = -(-(old + new) // PAGE)
+    total = int(have.sum()) + spare
+    ids = r.permutation(total)
+    table = np.full((len(old), max(1, int(have.max()))), -1)
+    at = 0
+    for b, h in enumerate(have):
+        table[b, :h] = ids[at:at + h]
+        at += h
+    pos = np.concatenate([old[b] + np.arange(new[b]) for b in range(len(old))] + [np.zeros(pad, int)]).astype(int)
+    rows = np.concatenate([np.full(new[b], b) for b in range(len(old))] + [np.full(pad, -1)]).astype(int)
+    slots = np.array([table[b, p // PAGE] * PAGE + p % PAGE if b >= 0 else -1 for b, p in zip(rows, pos)])
+    return pos, slots.astype(int), table, total
+
+
+def filled_cache(ops, pages, hkv, d, seed, garbage=True):
+    """Random codes (every byte, NaN too, where garbage) and scales."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    c = ops.paged_kv_cache(pages, hkv, d)
+    for t in (c.k, c.v):
+        b = torch.randint(0, 256, t.shape, generator=g, device="cuda", dtype=torch.int32).to(torch.uint8)
+        if not garbage:
+            b = torch.where((b & 0x7f) == 0x7f, b ^ 1, b)
+        t.view(torch.uint8).copy_(b)
+    for s in (c.k_scale, c.v_scale):
+        s.copy_(2.0 ** torch.randint(-9, -4, s.shape, generator=g, device="cuda").float())
+    return c
+
+
+def to_host(c):
+    return type(c)(*(t.cpu() for t in c))
+
+
+APPENDS = {
+    # old, new, hq, hkv, d, far (added to the rotation's positions), padding rows
+    "one token": ([0], [1], 4, 2, 128, 0, 0),
+    "decode": ([5, 63, 64, 127, 1000], [1] * 5, 8, 2, 128, 0, 0),
+    "prompt": ([0], [200], 4, 4, 128, 0, 0),
+    "continued": ([10, 64, 3], [150, 64, 61], 4, 1, 128, 0, 3),
+    "narrow": ([10, 0, 7], [150, 1, 2], 12, 2, 64, 0, 1),
+    "far positions": ([0, 60], [3, 70], 2, 2, 128, 1 << 20, 0),
+    "one head each": ([1], [5], 1, 1, 64, 0, 0),
+    "many heads": ([1, 2], [5, 1], 40, 8, 128, 0, 0),
+    "long batch": ([0, 70], [1500, 3], 4, 2, 128, 0, 5),
+}
+
+
+def check_append(ops, old, new, hq, hkv, d, far=0, pad=0, seed=0, mend=None, stride=0):
+    pos, slots, _, pages = layout(old, new, seed, pad=pad)
+    pos = pos + far
+    N = len(pos)
+    g = torch.Generator()
+    g.manual_seed(seed)
+    width = (hq + 2 * hkv) * d
+    qkv = (torch.randn(N, width + stride, generator=g) * (0.3 + 2 * torch.rand(width + stride, generator=g))).to(torch.bfloat16)
+    if mend:
+        mend(qkv)
+    qw, kw = ((1 + 0.1 * torch.randn(d, generator=g)).to(torch.bfloat16) for _ in range(2))
+    cache = filled_cache(ops, pages, hkv, d, seed)
+    before = to_host(type(cache)(*(t.clone() for t in cache)))
+    q_out = torch.full((N, hq, d), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.paged_qk_norm_rope_kv(qkv.cuda()[:, :width], qw.cuda(), kw.cuda(), dev(pos), dev(slots), ops.rope_turns(THETA, d),
+                              cache, q_out, hq, hkv, d, EPS)
+    after = to_host(cache)
+
+    x = qkv[:, :width].double().view(N, hq + 2 * hkv, d)
+    # fp32 against 64 bits: the mean of D squares, its root, two products and the turn each lose a few 2^-24 of the
+    # pair's size; the angle is off by 2^-25 turns + 2^-65 * position, 2^-22.3 radians: 2^-19 of the pair in all
+    q, size = oracle.norm_rope(x[:, :hq], qw.double(), pos, THETA, EPS)
+    assert torch.all((q_out.cpu().double() - q).abs() <= q.abs() * 2.0 ** -8 + size * 2.0 ** -18) or bool(mend)
+    k, size = oracle.norm_rope(x[:, hq:hq + hkv], kw.double(), pos, THETA, EPS)
+    v = x[:, hq + hkv:]
+    check_pages(before, after, k, v, size, slots, hkv)
+    return q_out, after
+
+
+def check_pages(before, after, k, v, size, slots, hkv):
+    bad = ~(k.isfinite().all(-1) & v.isfinite().all(-1))
+    touched = {}
+    for i, s in enumerate(slots):
+        if s >= 0:
+            touched.setdefault(int(s) // PAGE, []).append(i)
+    for page in range(before.k.shape[0]):
+        toks = touched.get(page, [])
+        offs = [int(slots[i]) % PAGE for i in toks]
+        for h in range(hkv):
+            for name, val, slack in (("k", k, size), ("v", v, None)):
+                codes_b, codes_a = getattr(before, name)[page, h], getattr(after, name)[page, h]
+                s_b, s_a = (float(getattr(c, name + "_scale")[page, h]) for c in (before, after))
+                if name == "v":
+                    codes_b, codes_a = codes_b.view(torch.uint8).T.view(torch.float8_e4m3fn), codes_a.view(torch.uint8).T.view(torch.float8_e4m3fn)
+                if not toks:
+                    assert torch.equal(codes_b.view(torch.uint8), codes_a.view(torch.uint8)) and s_a == s_b
+                    continue
+                good = [i for i in toks if not bad[i, h]]
+                amax = max([float(val[i, h].abs().max()) for i in good], default=0.0)
+                err = max([float(slack[i, h].max()) for i in good], default=0.0) * 2.0 ** -18 if slack is not None else 0.0
+                lo, hi = (oracle.scale_for(max(0.0, amax + e)) for e in (-err, err))
+                if min(offs) > 0:
+                    lo, hi = max(lo, s_b), max(hi, s_b)
+                assert lo <= s_a <= hi, (name, page, h, lo, s_a, hi)
+                # older tokens: their codes times the change of scale, rounded once more (exactly as a cast does)
+                first = min(offs)
+                old = (codes_b[:first].float() * (s_b / s_a)).to(torch.float8_e4m3fn)
+                assert torch.equal(old.float().nan_to_num(1e9), codes_a[:first].float().nan_to_num(1e9))
+                # slots that no token of the step has
+                rest = [o for o in range(first, PAGE) if o not in offs]
+                assert torch.equal(codes_b.view(torch.uint8)[rest], codes_a.view(torch.uint8)[rest])
+                for i, o in zip(toks, offs):
+                    got = codes_a[o].float().double() * s_a
+                    if bad[i, h]:
+                        assert got.isnan().all() if name == "k" else (got == 0).all()
+                        continue
+                    ref = val[i, h]
+                    # half a step: 2^-4 of the value, or half of the smallest code's 2^-9; a value past 448 is cut to it
+                    tol = ref.abs() * 2.0 ** -4 + 2.0 ** -10 * s_a + err
+                    assert torch.all((got - ref.clamp(-448 * s_a, 448 * s_a)).abs() <= tol), (name, page, h, o)
+
+
+@pytest.mark.parametrize("case", APPENDS, ids=list(APPENDS))
+def test_append(ops, case):
+    check_append(ops, *APPENDS[case])
+
+
+def test_append_strided_rows(ops):
+    check_append(ops, [3, 0], [70, 2], 4, 2, 128, stride=24)
+
+
+def test_append_raises_and_keeps_scales(ops):
+    """Tokens behind others: larger ones raise the page's scale, smaller ones leave it."""
+    for factor in (2.0 ** 9, 2.0 ** -9, 2.0 ** 40):
+        def mend(x, f=factor):
+            x *= f
+        check_append(ops, [7, 100], [3, 1], 4, 2, 128, mend=mend)
+
+
+def test_append_zeros(ops):
+    def mend(x):
+        x.zero_()
+    q, after = check_append(ops, [0, 3], [10, 4], 4, 2, 128, mend=mend)
+    assert (q.cpu() == 0).all()
+
+
+def test_append_not_finite(ops):
+    def mend(x):
+        d, hq, hkv = 128, 4, 2
+        x[2, (hq + 0) * d + 5] = math.nan             # K of head 0
+        x[3, (hq + hkv + 1) * d + 9] = math.inf       # V of head 1
+        x[70, (hq + 1) * d + 127] = -math.inf         # K of head 1
+    check_append(ops, [0], [80], 4, 2, 128, mend=mend)
+
+
+def test_append_huge_values(ops):
+    def mend(x):
+        x[:, 6 * 128:] = 3.3e38                       # V: past 448 * 2^119, cut to it
+        x[1, 6 * 128:] = -1e-38
+    check_append(ops, [0], [5], 4, 2, 128, mend=mend)
+
+
+def test_append_slots_outside_the_cache(ops):
+    """Rows whose slot is negative or past the last page append nothing; q is written for all."""
+    cache = filled_cache(ops, 3, 2, 128, 1)
+    before = [t.clone() for t in cache]
+    q_out = torch.zeros(4, 4, 128, dtype=torch.bfloat16, device="cuda")
+    qkv = torch.randn(4, 8 * 128, device="cuda").to(torch.bfloat16)
+    w = torch.ones(128, device="cuda", dtype=torch.bfloat16)
+    ops.paged_qk_norm_rope_kv(qkv, w, w, dev([0, 1, 2, 3]), dev([-1, 192, 2**31 - 1, -(2**31)]), ops.rope_turns(THETA, 128),
+                              cache, q_out, 4, 2, 128, EPS)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, cache))
+    assert (q_out != 0).any(-1).all()
+
+
+def test_append_nothing(ops):
+    cache = ops.paged_kv_cache(1, 1, 64)
+    e = lambda *s, dt=torch.bfloat16: torch.empty(*s, dtype=dt, device="cuda")  # noqa: E731
+    ops.paged_qk_norm_rope_kv(e(0, 192), e(64), e(64), e(0, dt=torch.int32), e(0, dt=torch.int32), ops.rope_turns(THETA, 64),
+                              cache, e(0, 1, 64), 1, 1, 64, EPS)
+
+
+# -------------------------------------------------------------- attention --
+ATTNS = {
+    # old, new, hq, hkv, d
+    "one key": ([0], [1], 4, 1, 128),
+    "single": ([8190], [1], 32, 8, 128),
+    "decode": ([0, 62, 63, 64, 200, 1], [1] * 6, 8, 2, 128),
+    "groups of one": ([100, 5], [1, 1], 4, 4, 64),
+    "group of five": ([130, 70], [1, 3], 10, 2, 128),
+    "group of sixteen": ([300], [1], 32, 2, 64),
+    "group of forty": ([70, 3], [2, 1], 40, 1, 64),
+    "a few each": ([100, 0, 64, 63], [5, 4, 2, 3], 8, 2, 128),
+    "rows of a tile's end": ([100, 30], [4, 8], 8, 2, 128),
+    "prompt": ([0], [300], 8, 2, 128),
+    "prompts": ([0, 0, 64], [65, 128, 191], 4, 4, 64),
+    "chunk beside decode": ([500, 77, 0, 200], [130, 1, 40, 1], 8, 2, 128),
+    "rows without tokens": ([10, 50, 0], [0, 2, 0], 4, 2, 128),
+    "ragged decode": ([3000, 1, 70, 900, 0, 511, 64, 2100], [1] * 8, 16, 2, 128),
+    "long chunk": ([700], [600], 4, 1, 128),
+    "wide rows": ([90], [100], 6, 2, 64),
+}
+
+
+def attention_case(ops, old, new, hq, hkv, d, seed=0, pad=3):
+    pos, slots, table, pages = layout(old, new, seed)
+    N = len(pos)
+    # garbage in every slot that no request has: NaN codes too.  Live slots hold finite codes
+    cache = filled_cache(ops, pages, hkv, d, seed)
+    live = torch.zeros(pages, PAGE, dtype=torch.bool)
+    for b in range(len(old)):
+        for p in range(old[b] + new[b]):
+            live[table[b, p // PAGE], p % PAGE] = True
+    for t, m in ((cache.k, live[:, None, :, None]), (cache.v, live[:, None, None, :])):
+        b = t.view(torch.uint8)
+        b.copy_(torch.where(m.cuda() & ((b & 0x7f) == 0x7f), b ^ 1, b))
+    # codes reach 448: with scales of 2^-9 .. 2^-5 keys of size 1 to 14, so that the softmax is peaked in places
+    g = torch.Generator()
+    g.manual_seed(seed + 1)
+    q = (torch.randn(N + pad, hq, d, generator=g) * 0.3).to(torch.bfloat16)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    return q, cache, table, cu, np.asarray(old) + np.asarray(new)
+
+
+def check_attention(ops, q, cache, table, cu, kv_lens, hq, hkv, d, scale=None, **kw):
+    scale = scale or 1 / math.sqrt(d)
+    out = torch.full((q.shape[0], hq * d), 5.0, dtype=torch.bfloat16, device="cuda")
+    got = ops.paged_attention(q.cuda(), cache, dev(table), dev(cu), dev(kv_lens), hq, hkv, d, scale, out=out, **kw)
+    assert got is out
+    hc = to_host(cache)
+    hc.k.view(torch.uint8).copy_(torch.where((hc.k.view(torch.uint8) & 0x7f) == 0x7f, 0, hc.k.view(torch.uint8)))
+    hc.v.view(torch.uint8).copy_(torch.where((hc.v.view(torch.uint8) & 0x7f) == 0x7f, 0, hc.v.view(torch.uint8)))
+    o, size = oracle.attention(q, hc, table, cu, kv_lens, hq, hkv, scale)
+    o, size = (x.reshape(len(q), -1) for x in (o, size))
+    end = int(cu[-1])
+    # each weight is rounded to bf16 (2^-8), the output too; scores in fp32: |q|.|k| scale is below 2^9 here and its D
+    # products and sums lose under 2^-19 of it, 2^-10 of a weight
+    tol = size * (2.0 ** -8 + 2.0 ** -9) + o.abs() * 2.0 ** -8 + 2.0 ** -100
+    diff = (out[:end].cpu().double() - o[:end]).abs()
+    assert torch.all(diff <= tol[:end]), float((diff / tol[:end]).max())
+    assert (out[end:] == 5.0).all()                   # rows behind the last request
+    return out
+
+
+@pytest.mark.parametrize("case", ATTNS, ids=list(ATTNS))
+def test_attention(ops, case):
+    old, new, hq, hkv, d = ATTNS[case]
+    args = attention_case(ops, old, new, hq, hkv, d)
+    a = check_attention(ops, *args, hq, hkv, d)
+    work = ops.paged_attention_workspace(len(args[0]), len(old), hq, hkv, d)
+    b = check_attention(ops, *args, hq, hkv, d, max_new=max(new), work=work)
+    c = check_attention(ops, *args, hq, hkv, d, max_new=max(new), work=work)
+    assert torch.equal(b, c)                          # the same bits again
+    assert a.shape == b.shape
+
+
+def test_attention_rows_that_see_nothing(ops):
+    """A request that was not admitted (no keys), and one with fewer keys than rows: zeros where no key is seen."""
+    q, cache, table, cu, kv = attention_case(ops, [10, 0, 20], [3, 5, 2], 4, 2, 128)
+    kv = np.array([13, 3, 0])
+    out = check_attention(ops, q, cache, table, cu, kv, 4, 2, 128)
+    assert (out[3:5] == 0).all() and (out[8:10] == 0).all() and (out[5:8] != 0).any()
+
+
+@pytest.mark.parametrize("new", [1, 50])
+def test_attention_bad_pages(ops, new):
+    """A page that the cache does not have counts as masked; a row left with none gives zeros."""
+    q, cache, table, cu, kv = attention_case(ops, [200, 300, 20], [new] * 3, 4, 2, 128)
+    table[0, 1], table[1, 0], table[1, 3] = -1, cache.k.shape[0], 2**31 - 1
+    table[2, :] = -5
+    out = check_attention(ops, q, cache, table, cu, kv, 4, 2, 128)
+    assert (out[2 * new:3 * new] == 0).all()
+
+
+def test_attention_shared_pages(ops):
+    """Two requests with the same prefix read the same pages."""
+    q, cache, table, cu, kv = attention_case(ops, [128, 128], [1, 1], 4, 2, 128)
+    table[1, :2] = table[0, :2]
+    check_attention(ops, q, cache, table, cu, kv, 4, 2, 128)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_nan_key(ops, new):
+    """A NaN key reaches exactly the rows that see it, in its head."""
+    q, cache, table, cu, kv = attention_case(ops, [70, 70], [new, new], 4, 2, 128)
+    at = 70 + new // 2 if new > 1 else 3              # a position in the chunk, or an old one
+    cache.k.view(torch.uint8)[table[0, at // PAGE], 1, at % PAGE, 17] = 0x7f
+    out = ops.paged_attention(q.cuda(), cache, dev(table), dev(cu), dev(kv), 4, 2, 128, 0.1).view(-1, 4, 128)
+    sees = torch.arange(new) + 70 >= at
+    assert out[:new, 2:][sees.cuda()].isnan().all()
+    rest = out.clone()
+    rest[:new, 2:][sees.cuda()] = 0
+    assert rest[:2 * new].isfinite().all()
+
+
+def test_attention_large_scores(ops):
+    """Scores far apart: the maximum moves along the pages and nothing overflows."""
+    q, cache, table, cu, kv = attention_case(ops, [300, 5], [1, 90], 4, 2, 128)
+    big = ops.PagedKV(cache.k, cache.v, cache.k_scale * 16, cache.v_scale)
+    # the scores reach thousands: fp32 keeps them to 2^-11, so compare with the oracle at the sizes of the values only
+    out = ops.paged_attention(q.cuda(), big, dev(table), dev(cu), dev(kv), 4, 2, 128, 1.0)
+    assert out[:91].isfinite().all()
+
+
+def test_attention_equal_scores(ops):
+    """q = 0: the mean of V, whatever the order of the pages."""
+    q, cache, table, cu, kv = attention_case(ops, [1000, 64], [1, 7], 4, 2, 128)
+    check_attention(ops, q * 0, cache, table, cu, kv, 4, 2, 128)
+
+
+def test_attention_nothing(ops):
+    cache = ops.paged_kv_cache(1, 1, 64)
+    out = ops.paged_attention(torch.empty(0, 1, 64, dtype=torch.bfloat16, device="cuda"), cache, dev([[0]]), dev([0, 0]),
+                              dev([0]), 1, 1, 64, 1.0)
+    assert out.shape == (0, 64)
+
+
+def test_attention_long_cache_offsets(ops):
+    """Pages whose bytes lie past 2^31 and 2^32 in the cache: 8 heads of 128, 8 KB a page and head and side."""
+    pages, hkv, d = 70000, 8, 128                     # 4.6 GB each of K and V
+    cache = ops.paged_kv_cache(pages, hkv, d)
+    used = [69999, 0, 33000, 66000]
+    ids = torch.tensor(used, device="cuda")
+    for t in (cache.k, cache.v):
+        b = torch.randint(0, 256, (4, *t.shape[1:]), device="cuda", dtype=torch.int32).to(torch.uint8)
+        t.view(torch.uint8)[ids] = torch.where((b & 0x7f) == 0x7f, b ^ 1, b)
+    cache.k_scale[ids], cache.v_scale[ids] = 2.0 ** -6, 2.0 ** -7
+    q = (torch.randn(40, 16, d) * 0.3).to(torch.bfloat16)
+    small = ops.PagedKV(*(t.view(torch.uint8)[ids].view(t.dtype) if t.dtype == torch.float8_e4m3fn else t[ids] for t in cache))
+    for n in (1, 40):
+        args = (q[:n].cuda().contiguous(),)
+        a = ops.paged_attention(*args, cache, dev([used]), dev([0, n]), dev([250]), 16, hkv, d, 0.1, max_new=n)
+        b = ops.paged_attention(*args, small, dev([[0, 1, 2, 3]]), dev([0, n]), dev([250]), 16, hkv, d, 0.1, max_new=n)
+        assert torch.equal(a, b)
+    # the append there, against the same append at the front
+    w = torch.ones(d, dtype=torch.bfloat16, device="cuda")
+    qkv = torch.randn(2, (16 + 2 * hkv) * d, device="cuda").to(torch.bfloat16)
+    qo = torch.empty(2, 16, d, dtype=torch.bfloat16, device="cuda")
+    for c, page in ((cache, 69999), (small, 0)):
+        ops.paged_qk_norm_rope_kv(qkv, w, w, dev([250, 251]), dev([page * 64 + 58, page * 64 + 59]), ops.rope_turns(THETA, d), c,
+                                  qo, 16, hkv, d, EPS)
+    for x, y in zip(cache, small):
+        assert torch.equal(x[69999].view(torch.uint8), y[0].view(torch.uint8))
+
+
+# --------------------------------------------------------------- together --
+def serve_step(ops, s, new, n):
+    """One step of a two-layer server on random activations: everything between the matrix products."""
+    plan = s["pool"].plan(new, n, out=s["plan"])
+    x = s["x"]
+    for layer in range(2):
+        qkv = torch.matmul(x, s["wqkv"][layer])
+        ops.paged_qk_norm_rope_kv(qkv, s["qw"], s["kw"], plan.positions, plan.slots, s["turns"], s["cache"][layer], s["q"],
+                                  s["hq"], s["hkv"], s["d"], EPS)
+        att = ops.paged_attention(s["q"], s["cache"][layer], s["pool"].table, plan.cu_q, plan.kv_lens, s["hq"], s["hkv"],
+                                  s["d"], 1 / math.sqrt(s["d"]), out=s["att"][layer], work=s["work"])
+        x = x + torch.matmul(att, s["wo"][layer])
+    logits = torch.matmul(x, s["lm"])
+    ops.sample(logits, s["u"], s["t"], s["k"], s["p"], s["mp"], tokens=s["tokens"], probs=s["probs"], work=s["swork"])
+    s["pool"].commit(plan, s["finished"])
+    return plan
+
+
+def server(ops, n, rows, pages=40, seed=0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    hq, hkv, d, hidden, vocab = 8, 2, 128, 256, 1000
+    rnd = lambda *sh: (torch.randn(*sh, generator=g, device="cuda") * sh[0] ** -0.5).to(torch.bfloat16)  # noqa: E731
+    f = lambda v, dt: torch.full((n,), v, dtype=dt, device="cuda")  # noqa: E731
+    pool = ops.PagePool(pages, rows, 8)
+    i = dict(dtype=torch.int32, device="cuda")
+    return dict(hq=hq, hkv=hkv, d=d, pool=pool, plan=ops.PagePlan(torch.zeros(rows + 1, **i), *(torch.zeros(rows, **i) for _ in range(2)),
+                                                                  *(torch.zeros(n, **i) for _ in range(2))),
+                x=rnd(n, hidden) * 16, wqkv=[rnd(hidden, (hq + 2 * hkv) * d) for _ in range(2)],
+                wo=[rnd(hq * d, hidden) for _ in range(2)], lm=rnd(hidden, vocab),
+                qw=torch.ones(d, dtype=torch.bfloat16, device="cuda"), kw=torch.ones(d, dtype=torch.bfloat16, device="cuda"),
+                turns=ops.rope_turns(THETA, d), cache=[filled_cache(ops, pages, hkv, d, seed) for _ in range(2)],
+                q=torch.zeros(n, hq, d, dtype=torch.bfloat16, device="cuda"),
+                att=[torch.zeros(n, hq * d, dtype=torch.bfloat16, device="cuda") for _ in range(2)],
+                work=ops.paged_attention_workspace(n, rows, hq, hkv, d), swork=ops.sample_workspace(n, vocab),
+                u=torch.rand(n, generator=g, device="cuda"), t=f(0.8, torch.float32), k=f(50, torch.int32), p=f(0.95, torch.float32),
+                mp=f(0.01, torch.float32), tokens=torch.zeros(n, dtype=torch.int64, device="cuda"),
+                probs=torch.zeros(n, device="cuda"), finished=torch.zeros(rows, dtype=torch.bool, device="cuda"))
+
+
+def test_steps_together(ops):
+    """Prompts, then decode beside a new prompt: each layer's attention is the oracle's over what the pages hold."""
+    s = server(ops, 200, 3)
+    for new in ([70, 0, 30], [1, 100, 1], [1, 1, 1], [0, 1, 66]):
+        before = host(s["pool"].lengths).copy()
+        s["x"].add_(0.125)                            # other tokens
+        plan = serve_step(ops, s, dev(new), 200)
+        n = sum(new)
+        assert np.array_equal(host(s["pool"].lengths), before + new)
+        for layer in range(2):
+            if layer == 1:                            # s["q"] holds the last layer's
+                c = to_host(s["cache"][layer])
+                for t in (c.k, c.v):
+                    t.view(torch.uint8).copy_(torch.where((t.view(torch.uint8) & 0x7f) == 0x7f, 0, t.view(torch.uint8)))
+                o, size = oracle.attention(s["q"].cpu(), c, host(s["pool"].table), host(plan.cu_q), host(plan.kv_lens), 8, 2, 1 / math.sqrt(128))
+                o, size = o.reshape(200, -1), size.reshape(200, -1)
+                tol = size * (2.0 ** -8 + 2.0 ** -9) + o.abs() * 2.0 ** -8 + 2.0 ** -100
+                assert torch.all((s["att"][layer].cpu().double() - o).abs()[:n] <= tol[:n])
+        assert (host(s["tokens"])[:n] >= 0).all() and (host(s["tokens"])[:n] < 1000).all()
+
+
+def test_captured_step_replays(ops):
+    """A captured decode step against the same steps run eagerly, with eager work and synchronisations in between."""
+    a, b = server(ops, 4, 4, seed=3), server(ops, 4, 4, seed=3)
+    new = dev([1, 1, 0, 1])
+    for s in (a, b):                                  # also the warm-up of the library's products
+        for _ in range(3):
+            serve_step(ops, s, new, 4)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        serve_step(ops, a, new, 4)
+    for step in range(70):                            # over a page border
+        for s in (a, b):
+            s["x"].add_(0.0625)
+        g.replay()
+        if step % 7 == 3:
+            torch.cuda.synchronize()
+        serve_step(ops, b, new, 4)
+        if step % 5 == 0:
+            assert torch.equal(a["tokens"], b["tokens"]) and torch.equal(a["att"][1][:3], b["att"][1][:3])
+            assert torch.equal(a["probs"], b["probs"])
+    assert torch.equal(a["pool"].lengths, b["pool"].lengths) and host(a["pool"].lengths).tolist() == [73, 73, 0, 73]
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for p, q in zip(a["cache"], b["cache"]) for x, y in zip(p, q))
+
+
+def test_two_streams(ops):
+    """Calls on two streams at once, each with buffers of its own, give what they give alone."""
+    servers = [server(ops, 64, 4, seed=i) for i in (1, 2)]
+    new = dev([16, 16, 16, 16])
+    want = []
+    for i in (1, 2):
+        s = server(ops, 64, 4, seed=i)
+        for _ in range(5):
+            serve_step(ops, s, new, 64)
+        want.append((s["att"][1].clone(), s["tokens"].clone()))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for st, s in zip(streams, servers):
+            with torch.cuda.stream(st):
+                serve_step(ops, s, new, 64)
+    torch.cuda.synchronize()
+    for s, (att, tok) in zip(servers, want):
+        assert torch.equal(s["att"][1], att) and torch.equal(s["tokens"], tok)
