@@ -29,26 +29,45 @@ PAGE = 64            # tokens of a page (csrc/ops/paged.h)
 MAX_ROWS = 1024      # requests of one call
 
 
-def _on(device: torch.device, name: str, **tensors):
-    """Every tensor on ``device``, of its type, contiguous: ``name=(tensor, dtype)``."""
-    if device.type != "cuda":
-        raise ValueError(f"{name}: tensors must be on the GPU, got {device}")
-    for what, (t, dtype) in tensors.items():
+_I32, _I64, _F32, _BF16, _FP8 = torch.int32, torch.int64, torch.float32, torch.bfloat16, torch.float8_e4m3fn
+
+
+def _ptrs(name: str, *specs):
+    """Device index and addresses of ``(what, tensor or None, dtype, shape)``: each contiguous, of its type and shape,
+    all on one GPU.  (A fraction of a microsecond a tensor: a decode step makes these calls for every layer.)"""
+    idx, out = None, []
+    for what, t, dtype, shape in specs:
         if t is None:
+            out.append(None)
             continue
-        if t.device != device or t.dtype != dtype or not t.is_contiguous():
-            raise ValueError(f"{name}: {what} must be contiguous {dtype} on {device}, got "
-                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
+        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name}: {what} must be contiguous {dtype} {list(shape)}, got {t.dtype} {list(t.shape)} "
+                             f"strides {list(t.stride())}")
+        d = t.get_device()
+        if idx is None:
+            idx = d
+        if d != idx or d < 0:
+            raise ValueError(f"{name}: {what} is on {t.device}: every tensor must be on one GPU")
+        out.append(t.data_ptr())
+    return idx, out
 
 
-def _launch(device, name, fn, *args):
-    """The C call on ``device``'s current stream, whatever the current device is."""
-    with torch.cuda.device(device):
-        ops._check(fn(*args, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)), name)
+def _launch(idx: int, name: str, fn, *args):
+    """The C call on the current stream of the tensors' GPU, whatever the current device is."""
+    if idx == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if rc == -2:
+        raise ValueError(f"{name}: the workspace is too small for this call")
+    ops._check(rc, name)
 
 
-def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+def _aligned(name: str, **ptrs):
+    for what, p in ptrs.items():
+        if p % 16:
+            raise ValueError(f"{name}: {what} must start at a multiple of 16 bytes")
 
 
 # ------------------------------------------------------------------ pages --
@@ -78,28 +97,22 @@ def page_plan(new_lens: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
     if its tokens fit (64 * W of them, and ``n_tokens`` rows in all) and the free pages reach for the pages of every
     request up to it; what it would have taken stays reserved for it ahead of later ones.  Nothing that is committed
     changes: planning again gives the same plan, and ``page_commit`` makes it so."""
-    B = new_lens.numel()
-    dev = new_lens.device
-    i32 = torch.int32
-    _on(dev, "page_plan", new_lens=(new_lens, i32), lengths=(lengths, i32), table=(table, i32), free=(free, i32),
-        ring=(ring, i32))
-    if not 0 < B <= MAX_ROWS or new_lens.dim() != 1 or tuple(lengths.shape) != (B,) or table.dim() != 2 \
-            or table.shape[0] != B or table.shape[1] < 1 or free.dim() != 1 or free.numel() < 1 or tuple(ring.shape) != (2,):
-        raise ValueError(f"page_plan: new_lens / lengths [B <= {MAX_ROWS}], table [B, W], free [pages], ring [2]; got "
-                         f"{tuple(new_lens.shape)} {tuple(lengths.shape)} {tuple(table.shape)} {tuple(free.shape)} "
-                         f"{tuple(ring.shape)}")
-    if n_tokens < 0 or max(free.numel(), table.shape[1]) * PAGE > 2**31 - 1:
-        raise ValueError(f"page_plan: n_tokens {n_tokens}, {free.numel()} pages, {table.shape[1]} a request: slots are "
-                         "32-bit")
+    if table.dim() != 2 or not 0 < table.shape[0] <= MAX_ROWS or table.shape[1] < 1 or free.dim() != 1 \
+            or free.numel() < 1:
+        raise ValueError(f"page_plan: table [B <= {MAX_ROWS}, W], free [pages], got {list(table.shape)} {list(free.shape)}")
+    B, W = table.shape
+    pages = free.numel()
+    if n_tokens < 0 or max(pages, W) * PAGE > 2**31 - 1:
+        raise ValueError(f"page_plan: n_tokens {n_tokens}, {pages} pages, {W} a request: slots are 32-bit")
     if out is None:
-        buf = torch.empty(3 * B + 1 + 2 * n_tokens, dtype=i32, device=dev)     # one allocation
-        out = PagePlan(*buf.split([B + 1, B, B, n_tokens, n_tokens]))
-    else:
-        _on(dev, "page_plan", **{n: (t, i32) for n, t in zip(PagePlan._fields, out)})
-        if [t.numel() for t in out] != [B + 1, B, B, n_tokens, n_tokens]:
-            raise ValueError(f"page_plan: out must hold {B + 1}, {B}, {B}, {n_tokens}, {n_tokens} values")
-    _launch(dev, "page_plan", ops.lib().mivgpu_page_plan, _ptr(new_lens), _ptr(lengths), _ptr(table), _ptr(free),
-            _ptr(ring), *map(_ptr, out), B, table.shape[1], free.numel(), n_tokens)
+        buf = torch.empty(3 * B + 1 + 2 * n_tokens, dtype=_I32, device=table.device)     # one allocation
+        out = PagePlan(*torch.split_with_sizes(buf, (B + 1, B, B, n_tokens, n_tokens)))
+    idx, p = _ptrs("page_plan", ("new_lens", new_lens, _I32, (B,)), ("lengths", lengths, _I32, (B,)),
+                   ("table", table, _I32, (B, W)), ("free", free, _I32, (pages,)), ("ring", ring, _I32, (2,)),
+                   ("cu_q", out.cu_q, _I32, (B + 1,)), ("kv_lens", out.kv_lens, _I32, (B,)),
+                   ("taken", out.taken, _I32, (B,)), ("positions", out.positions, _I32, (n_tokens,)),
+                   ("slots", out.slots, _I32, (n_tokens,)))
+    _launch(idx, "page_plan", ops.lib().mivgpu_page_plan, *p, B, W, pages, n_tokens)
     return out
 
 
@@ -107,17 +120,15 @@ def page_commit(plan: PagePlan, lengths: torch.Tensor, table: torch.Tensor, free
                 finished: torch.Tensor | None = None):
     """The plan's step is done: ``lengths`` of admitted requests become its ``kv_lens`` and their pages leave the
     ring.  ``finished`` (bool [B]): requests whose pages go back to the ring's end, in order; their length becomes 0."""
-    B = lengths.numel()
-    dev = lengths.device
-    i32 = torch.int32
-    _on(dev, "page_commit", lengths=(lengths, i32), table=(table, i32), free=(free, i32), ring=(ring, i32),
-        kv_lens=(plan.kv_lens, i32), taken=(plan.taken, i32), finished=(finished, torch.bool))
-    if not 0 < B <= MAX_ROWS or lengths.dim() != 1 or tuple(plan.kv_lens.shape) != (B,) or tuple(plan.taken.shape) != (B,) \
-            or table.dim() != 2 or table.shape[0] != B or free.dim() != 1 or free.numel() < 1 \
-            or tuple(ring.shape) != (2,) or (finished is not None and tuple(finished.shape) != (B,)):
-        raise ValueError(f"page_commit: a plan, table and finished of {B} requests, free [pages], ring [2]")
-    _launch(dev, "page_commit", ops.lib().mivgpu_page_commit, _ptr(plan.kv_lens), _ptr(plan.taken), _ptr(finished),
-            _ptr(lengths), _ptr(table), _ptr(free), _ptr(ring), B, table.shape[1], free.numel())
+    if table.dim() != 2 or not 0 < table.shape[0] <= MAX_ROWS or table.shape[1] < 1 or free.dim() != 1 \
+            or free.numel() < 1 or max(free.numel(), table.shape[1]) * PAGE > 2**31 - 1:
+        raise ValueError(f"page_commit: table [B <= {MAX_ROWS}, W], free [pages], got {list(table.shape)} {list(free.shape)}")
+    B, W = table.shape
+    pages = free.numel()
+    idx, p = _ptrs("page_commit", ("kv_lens", plan.kv_lens, _I32, (B,)), ("taken", plan.taken, _I32, (B,)),
+                   ("finished", finished, torch.bool, (B,)), ("lengths", lengths, _I32, (B,)),
+                   ("table", table, _I32, (B, W)), ("free", free, _I32, (pages,)), ("ring", ring, _I32, (2,)))
+    _launch(idx, "page_commit", ops.lib().mivgpu_page_commit, *p, B, W, pages)
 
 
 class PagePool:
@@ -160,21 +171,17 @@ def paged_kv_cache(num_pages: int, n_kv_heads: int, head_dim: int, device="cuda"
                    torch.empty(num_pages, n_kv_heads, **scale), torch.empty(num_pages, n_kv_heads, **scale))
 
 
-def _check_cache(cache: PagedKV, device, name, n_q_heads, n_kv_heads, head_dim) -> int:
-    """Host check of the cache's layout and the head counts; returns its pages."""
+def _cache_specs(cache: PagedKV, name: str, n_q_heads: int, n_kv_heads: int, head_dim: int):
+    """Host check of the head counts; the cache's pages and what ``_ptrs`` checks of it."""
     if n_kv_heads < 1 or n_q_heads < 1 or n_q_heads % n_kv_heads or head_dim not in (64, 128):
         raise ValueError(f"{name}: {n_q_heads} / {n_kv_heads} heads of {head_dim} (64 or 128)")
-    _on(device, name, k=(cache.k, torch.float8_e4m3fn), v=(cache.v, torch.float8_e4m3fn),
-        k_scale=(cache.k_scale, torch.float32), v_scale=(cache.v_scale, torch.float32))
     pages = cache.k.shape[0]
-    if tuple(cache.k.shape) != (pages, n_kv_heads, PAGE, head_dim) or tuple(cache.v.shape) != (pages, n_kv_heads, head_dim, PAGE) \
-            or tuple(cache.k_scale.shape) != (pages, n_kv_heads) or tuple(cache.v_scale.shape) != (pages, n_kv_heads):
-        raise ValueError(f"{name}: cache k {tuple(cache.k.shape)}, v {tuple(cache.v.shape)}, scales "
-                         f"{tuple(cache.k_scale.shape)} {tuple(cache.v_scale.shape)} do not match {n_kv_heads} heads of "
-                         f"{head_dim}")
     if pages < 1 or pages * PAGE > 2**31 - 1:
         raise ValueError(f"{name}: {pages} pages: slots are 32-bit")
-    return pages
+    return pages, (("k", cache.k, _FP8, (pages, n_kv_heads, PAGE, head_dim)),
+                   ("v", cache.v, _FP8, (pages, n_kv_heads, head_dim, PAGE)),
+                   ("k_scale", cache.k_scale, _F32, (pages, n_kv_heads)),
+                   ("v_scale", cache.v_scale, _F32, (pages, n_kv_heads)))
 
 
 # ----------------------------------------------------------------- append --
@@ -197,39 +204,41 @@ def paged_qk_norm_rope_kv(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: t
     in the order of their slots, behind the page's live tokens: a page whose first slot is written starts afresh, any
     other keeps its earlier tokens, whose codes follow when a new value raises the page's scale.  (``PagePool.plan``
     gives such slots.)  A token whose K or V of a head is not finite is stored as NaN in K and zero in V."""
-    N = positions.numel()
-    dev = qkv.device
-    pages = _check_cache(cache, dev, "paged_qk_norm_rope_kv", n_q_heads, n_kv_heads, head_dim)
-    bf = torch.bfloat16
+    name = "paged_qk_norm_rope_kv"
+    pages, specs = _cache_specs(cache, name, n_q_heads, n_kv_heads, head_dim)
     width = (n_q_heads + 2 * n_kv_heads) * head_dim
-    _on(dev, "paged_qk_norm_rope_kv", q_norm_w=(q_norm_w, bf), k_norm_w=(k_norm_w, bf), positions=(positions, torch.int32),
-        slots=(slots, torch.int32), turns=(turns, torch.int64), q_out=(q_out, bf))
-    if qkv.dtype != bf or qkv.dim() != 2 or tuple(qkv.shape) != (N, width) or (N > 0 and qkv.stride(1) != 1) \
+    N = positions.shape[0] if positions.dim() == 1 else -1
+    if qkv.dtype is not _BF16 or qkv.shape != (N, width) or (N > 0 and qkv.stride(1) != 1) \
             or (N > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < width)):
-        raise ValueError(f"paged_qk_norm_rope_kv: qkv must be bf16 [{N}, {width}] with unit column stride and a row stride "
-                         f"that is a multiple of 8, got {tuple(qkv.shape)} {qkv.dtype} strides {qkv.stride()}")
-    if tuple(positions.shape) != (N,) or tuple(slots.shape) != (N,) or q_norm_w.numel() != head_dim \
-            or k_norm_w.numel() != head_dim or turns.numel() != head_dim // 2 \
-            or tuple(q_out.shape) != (N, n_q_heads, head_dim):
-        raise ValueError(f"paged_qk_norm_rope_kv: positions / slots [{N}], norm weights [{head_dim}], turns "
-                         f"[{head_dim // 2}], q_out [{N}, {n_q_heads}, {head_dim}]")
-    for what, t in (("qkv", qkv), ("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w), ("q_out", q_out), ("k", cache.k),
-                    ("v", cache.v)):
-        if N > 0 and t.data_ptr() % 16:
-            raise ValueError(f"paged_qk_norm_rope_kv: {what} must start at a multiple of 16 bytes")
-    _launch(dev, "paged_qk_norm_rope_kv", ops.lib().mivgpu_paged_qk_norm_rope_kv, _ptr(qkv),
-            qkv.stride(0) if N > 1 else width, _ptr(q_norm_w), _ptr(k_norm_w), _ptr(positions), _ptr(slots), _ptr(turns),
-            _ptr(q_out), _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), N, n_q_heads, n_kv_heads,
-            head_dim, pages, eps)
+        raise ValueError(f"{name}: qkv must be bf16 [{N}, {width}] with unit column stride and a row stride that is a "
+                         f"multiple of 8, got {qkv.dtype} {list(qkv.shape)} strides {list(qkv.stride())}")
+    idx, p = _ptrs(name, ("q_norm_w", q_norm_w, _BF16, (head_dim,)), ("k_norm_w", k_norm_w, _BF16, (head_dim,)),
+                   ("positions", positions, _I32, (N,)), ("slots", slots, _I32, (N,)),
+                   ("turns", turns, _I64, (head_dim // 2,)), ("q_out", q_out, _BF16, (N, n_q_heads, head_dim)), *specs)
+    if qkv.get_device() != idx:
+        raise ValueError(f"{name}: qkv is on {qkv.device}: every tensor must be on one GPU")
+    _aligned(name, qkv=qkv.data_ptr(), q_norm_w=p[0], k_norm_w=p[1], q_out=p[5], k=p[6], v=p[7])
+    _launch(idx, name, ops.lib().mivgpu_paged_qk_norm_rope_kv, qkv.data_ptr(), qkv.stride(0) if N > 1 else width, *p, N,
+            n_q_heads, n_kv_heads, head_dim, pages, eps)
     return q_out
 
 
 # -------------------------------------------------------------- attention --
 def paged_attention_workspace(n_tokens: int, rows: int, n_q_heads: int, n_kv_heads: int, head_dim: int,
                               device="cuda") -> torch.Tensor:
-    """Workspace of ``paged_attention`` for steps of up to ``n_tokens`` tokens and ``rows`` requests.  Calls that may
-    run at once (two streams, two captured graphs replayed side by side) need one each."""
-    return torch.empty(0, dtype=torch.float32, device=device)
+    """Workspace of ``paged_attention`` for steps of up to ``n_tokens`` tokens and ``rows`` requests: room for the parts
+    that a long request is split into, and counters that every call leaves at zero.  Calls that may run at once (two
+    streams, two captured graphs replayed side by side) need one each."""
+    if n_tokens < 0 or not 0 < rows <= MAX_ROWS or n_kv_heads < 1 or n_q_heads < 1 or n_q_heads % n_kv_heads \
+            or head_dim not in (64, 128):
+        raise ValueError(f"paged_attention_workspace: {n_tokens} tokens of {rows} requests, {n_q_heads} / {n_kv_heads} "
+                         f"heads of {head_dim} (64 or 128)")
+    zeroed = ctypes.c_longlong(0)
+    with torch.cuda.device(device):
+        floats = ops.lib().mivgpu_paged_attention_work(n_tokens, rows, n_q_heads, n_kv_heads, head_dim, ctypes.byref(zeroed))
+    work = torch.empty(floats, dtype=_F32, device=device)
+    work[:zeroed.value].zero_()
+    return work
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKV, table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor,
@@ -241,28 +250,24 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, table: torch.Tensor, cu_q: 
     table[b] (int32 [B, W], B <= 1024).  A row that sees no key (a request with kv_lens 0) gives zeros; rows behind
     cu_q[B] are left as they are; keys on a page that the cache does not have count as masked.  ``max_new``: the most
     new tokens of a request, if known (1 in a decode step).  ``work`` from ``paged_attention_workspace``."""
+    name = "paged_attention"
+    pages, specs = _cache_specs(cache, name, n_q_heads, n_kv_heads, head_dim)
     N = q.shape[0]
-    B = kv_lens.numel()
-    dev = q.device
-    pages = _check_cache(cache, dev, "paged_attention", n_q_heads, n_kv_heads, head_dim)
-    i32, bf = torch.int32, torch.bfloat16
-    if out is None:
-        out = torch.zeros(N, n_q_heads * head_dim, dtype=bf, device=dev)
-    _on(dev, "paged_attention", q=(q, bf), table=(table, i32), cu_q=(cu_q, i32), kv_lens=(kv_lens, i32), out=(out, bf),
-        work=(work, torch.float32))
-    if tuple(q.shape) != (N, n_q_heads, head_dim) or tuple(out.shape) != (N, n_q_heads * head_dim):
-        raise ValueError(f"paged_attention: q {tuple(q.shape)}, out {tuple(out.shape)} do not match {n_q_heads} heads of "
-                         f"{head_dim}")
-    if not 0 < B <= MAX_ROWS or tuple(kv_lens.shape) != (B,) or tuple(cu_q.shape) != (B + 1,) or table.dim() != 2 \
-            or table.shape[0] != B or table.shape[1] < 1:
-        raise ValueError(f"paged_attention: kv_lens [B <= {MAX_ROWS}], cu_q [B + 1], table [B, W]; got "
-                         f"{tuple(kv_lens.shape)} {tuple(cu_q.shape)} {tuple(table.shape)}")
+    if table.dim() != 2 or not 0 < table.shape[0] <= MAX_ROWS or table.shape[1] < 1 or table.shape[1] * PAGE > 2**31 - 1:
+        raise ValueError(f"{name}: table must be [B <= {MAX_ROWS}, W], got {list(table.shape)}")
     if max_new is not None and max_new < 0:
-        raise ValueError(f"paged_attention: max_new {max_new}")
-    for what, t in (("q", q), ("out", out), ("k", cache.k), ("v", cache.v)):
-        if N > 0 and t.data_ptr() % 16:
-            raise ValueError(f"paged_attention: {what} must start at a multiple of 16 bytes")
-    _launch(dev, "paged_attention", ops.lib().mivgpu_paged_attention, _ptr(q), _ptr(cache.k), _ptr(cache.v),
-            _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(table), _ptr(cu_q), _ptr(kv_lens), _ptr(out), N, B,
-            table.shape[1], n_q_heads, n_kv_heads, head_dim, pages, scale)
+        raise ValueError(f"{name}: max_new {max_new}")
+    B, W = table.shape
+    if out is None:
+        out = torch.zeros(N, n_q_heads * head_dim, dtype=_BF16, device=q.device)
+    idx, p = _ptrs(name, ("q", q, _BF16, (N, n_q_heads, head_dim)), *specs, ("table", table, _I32, (B, W)),
+                   ("cu_q", cu_q, _I32, (B + 1,)), ("kv_lens", kv_lens, _I32, (B,)),
+                   ("out", out, _BF16, (N, n_q_heads * head_dim)))
+    if work is None:
+        work = paged_attention_workspace(N, B, n_q_heads, n_kv_heads, head_dim, q.device)
+    if work.dtype is not _F32 or work.dim() != 1 or not work.is_contiguous() or work.get_device() != idx:
+        raise ValueError(f"{name}: work must be from paged_attention_workspace on {q.device}")
+    _aligned(name, q=p[0], k=p[1], v=p[2], out=p[8], work=work.data_ptr())
+    _launch(idx, name, ops.lib().mivgpu_paged_attention, *p, work.data_ptr(), work.numel(), N, B, W, n_q_heads, n_kv_heads,
+            head_dim, pages, scale)
     return out

@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from k8s_vgpu_scheduler_amd import ops
-from k8s_vgpu_scheduler_amd.ops.paged import _launch, _on, _ptr
+from k8s_vgpu_scheduler_amd.ops.paged import _BF16, _F32, _I32, _I64, _launch, _ptrs
 
 MAX_VOCAB = 128 * 32768      # csrc/ops/sample.hip CARRIES * CHUNK
 
@@ -31,22 +31,18 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tenso
     if logits.dim() != 2:
         raise ValueError(f"sample: logits must be [B, V], got {tuple(logits.shape)}")
     B, V = logits.shape
-    dev = logits.device
-    if logits.dtype != torch.bfloat16 or B < 1 or not 0 < V <= MAX_VOCAB or (V > 1 and logits.stride(1) != 1) \
+    if logits.dtype is not _BF16 or B < 1 or not 0 < V <= MAX_VOCAB or (V > 1 and logits.stride(1) != 1) \
             or (B > 1 and logits.stride(0) < V):
         raise ValueError(f"sample: logits must be bf16 [B, V <= {MAX_VOCAB}] with unit column stride, got "
-                         f"{tuple(logits.shape)} {logits.dtype} strides {logits.stride()}")
+                         f"{logits.dtype} {list(logits.shape)} strides {list(logits.stride())}")
     if tokens is None:
-        tokens = torch.empty(B, dtype=torch.int64, device=dev)
+        tokens = torch.empty(B, dtype=_I64, device=logits.device)
     if probs is None:
-        probs = torch.empty(B, dtype=torch.float32, device=dev)
-    f32 = torch.float32
-    rows = dict(uniform=(uniform, f32), temperature=(temperature, f32), top_k=(top_k, torch.int32), top_p=(top_p, f32),
-                min_p=(min_p, f32), tokens=(tokens, torch.int64), probs=(probs, f32))
-    _on(dev, "sample", **rows, work=(work, torch.int64))
-    for what, (t, _) in rows.items():
-        if t is not None and tuple(t.shape) != (B,):
-            raise ValueError(f"sample: {what} must have one value a row ({B}), got {tuple(t.shape)}")
-    _launch(dev, "sample", ops.lib().mivgpu_sample, _ptr(logits), logits.stride(0) if B > 1 else V, V, B, _ptr(uniform),
-            _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(tokens), _ptr(probs))
+        probs = torch.empty(B, dtype=_F32, device=logits.device)
+    idx, p = _ptrs("sample", ("uniform", uniform, _F32, (B,)), ("temperature", temperature, _F32, (B,)),
+                   ("top_k", top_k, _I32, (B,)), ("top_p", top_p, _F32, (B,)), ("min_p", min_p, _F32, (B,)),
+                   ("tokens", tokens, _I64, (B,)), ("probs", probs, _F32, (B,)))
+    if logits.get_device() != idx:
+        raise ValueError(f"sample: logits are on {logits.device}: every tensor must be on one GPU")
+    _launch(idx, "sample", ops.lib().mivgpu_sample, logits.data_ptr(), logits.stride(0) if B > 1 else V, V, B, *p)
     return tokens, probs
