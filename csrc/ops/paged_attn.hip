@@ -30,6 +30,7 @@ typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 
 constexpr int NT = 256, WAVES = 4, TILE = 16;
 constexpr int MIN_CHUNK = WAVES;         // pages of a part: at least one for each wave
+constexpr int MAX_PARTS = 256;           // of a tile: their (m, l) take 32 KB of LDS
 
 // 8 codes -> 8 bf16, times 2^e
 __device__ __forceinline__ bf16x8_t widen(uint32_t lo, uint32_t hi, float s) {
@@ -63,8 +64,69 @@ __device__ __forceinline__ void store_row(bf16_t* out, f32x4_t o, float l, int r
   *reinterpret_cast<uint2*>(at) = make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv));
 }
 
+// which request, tile of its rows and part of that tile's pages a workgroup takes, from its index among all parts
+struct Share {
+  int b, tile, part, ns;     // ns: parts of the tile; 0: nothing left for this workgroup
+};
+
+// Every wave scans all requests by itself (contiguous ones in a lane): no barrier, and one round of loads for up to
+// 64 requests.
+__device__ __forceinline__ Share find_share(const int* __restrict__ cu, const int* __restrict__ kv_lens, int N, int B, int W,
+                                            int G, int target) {
+  const int lane = threadIdx.x & 63, per = (B + 63) / 64;
+  auto size = [&](int b, int* tiles, int* np) {
+    *tiles = *np = 0;
+    if (b < B) {
+      const int n = max(min(cu[b + 1], N) - min(max(cu[b], 0), N), 0);
+      *tiles = (n * G + TILE - 1) / TILE;
+      *np = (min(max(kv_lens[b], 0), W * PAGE) + PAGE - 1) / PAGE;
+    }
+  };
+  int tiles, np;
+  long long sum = 0;
+  for (int i = 0; i < per; ++i) {
+    size(lane * per + i, &tiles, &np);
+    sum += (long long)tiles * np;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  const int chunk = (int)max((sum + target - 1) / target, (long long)MIN_CHUNK);
+  auto parts = [&](int np) { return min(max((np + chunk - 1) / chunk, 1), MAX_PARTS); };
+  sum = 0;
+  for (int i = 0; i < per; ++i) {
+    size(lane * per + i, &tiles, &np);
+    sum += (long long)tiles * parts(np);
+  }
+  long long at = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long long u = __shfl_up(at, o, 64);
+    if (lane >= o) at += u;
+  }
+  at -= sum;
+  const unsigned long long owner = __ballot((long long)blockIdx.x >= at && (long long)blockIdx.x < at + sum);
+  Share sh = {0, 0, 0, 0};
+  if (owner == 0) return sh;
+  const int who = __ffsll((long long)owner) - 1;
+  int x = (int)(blockIdx.x - __shfl(at, who, 64));
+  for (int i = 0; i < per; ++i) {
+    size(who * per + i, &tiles, &np);
+    const int ns = parts(np);
+    if ((long long)x < (long long)tiles * ns) {
+      sh.b = who * per + i, sh.tile = x / ns, sh.part = x % ns, sh.ns = ns;
+      break;
+    }
+    x -= tiles * ns;
+  }
+  sh.b = __builtin_amdgcn_readfirstlane(sh.b);
+  sh.tile = __builtin_amdgcn_readfirstlane(sh.tile);
+  sh.part = __builtin_amdgcn_readfirstlane(sh.part);
+  sh.ns = __builtin_amdgcn_readfirstlane(sh.ns);
+  return sh;
+}
+
 template <int D>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, 3)
 attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
             const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ table,
             const int* __restrict__ cu, const int* __restrict__ kv_lens, bf16_t* __restrict__ out,
@@ -72,56 +134,18 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
             int Hq, int Hkv, int pages, int target, float scale_log2) {
   constexpr int KU = D / 64;              // 16-byte chunks of a K row per lane
   constexpr int DT = D / 16;              // output tiles
-  __shared__ long long red[WAVES];
-  __shared__ int s_b, s_tile, s_part, s_ns, s_first;
   __shared__ float s_m[WAVES][TILE], s_l[WAVES][TILE];
-  __shared__ __attribute__((aligned(16))) float s_o[WAVES][TILE][D + 4];
+  // the waves' O; later the (m, l) of a tile's parts and what groups of threads make of them
+  constexpr int O_BYTES = WAVES * TILE * (D + 4) * 4, JOIN_BYTES = MAX_PARTS * TILE * 8 + NT * 20;
+  __shared__ __attribute__((aligned(16))) char s_raw[O_BYTES > JOIN_BYTES ? O_BYTES : JOIN_BYTES];
+  float(*s_o)[TILE][D + 4] = reinterpret_cast<float(*)[TILE][D + 4]>(s_raw);
+  __shared__ int s_last;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 15, a = lane >> 4;
   const int G = Hq / Hkv, hk = blockIdx.y;
-
-  // which request, tile and part: the workgroup's index among all tiles' parts
-  {
-    constexpr int PER = MAX_ROWS / NT;
-    int tiles[PER], np[PER];
-    long long sum = 0, all;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int b = t * PER + i;
-      tiles[i] = np[i] = 0;
-      if (b < B) {
-        const int n = max(min(cu[b + 1], N) - min(max(cu[b], 0), N), 0);
-        tiles[i] = (n * G + TILE - 1) / TILE;
-        np[i] = (min(max(kv_lens[b], 0), W * PAGE) + PAGE - 1) / PAGE;
-      }
-      sum += (long long)tiles[i] * np[i];
-    }
-    block_scan<NT>(sum, red, &all);
-    const int chunk = (int)max((all + target - 1) / target, (long long)MIN_CHUNK);
-    sum = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      np[i] = max((np[i] + chunk - 1) / chunk, 1);       // now parts of a tile
-      sum += (long long)tiles[i] * np[i];
-    }
-    long long at = block_scan<NT>(sum, red, &all) - sum;
-    if ((long long)blockIdx.x >= all) return;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const long long mine = (long long)tiles[i] * np[i];
-      if (blockIdx.x >= at && blockIdx.x < at + mine) {
-        const int x = (int)(blockIdx.x - at);
-        s_b = t * PER + i;
-        s_tile = x / np[i];
-        s_part = x % np[i];
-        s_ns = np[i];
-        s_first = (int)blockIdx.x - s_part;
-      }
-      at += mine;
-    }
-    __syncthreads();
-  }
-  const int b = s_b, row0 = s_tile * TILE, ns = s_ns, first = s_first;
+  const Share sh = find_share(cu, kv_lens, N, B, W, G, target);
+  if (sh.ns == 0) return;
+  const int b = sh.b, row0 = sh.tile * TILE, ns = sh.ns;
   const int tok0 = min(max(cu[b], 0), N), n = min(cu[b + 1], N) - tok0, rows = n * G;
   const int L = min(max(kv_lens[b], 0), W * PAGE);
 
@@ -149,16 +173,24 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
   float m = -INFINITY, l = 0.f;
 
   const int npages = (most + PAGE - 1) / PAGE;
-  const int p0 = (int)((long long)npages * s_part / ns), p1 = (int)((long long)npages * (s_part + 1) / ns);
-  for (int p = p0 + w; p < p1; p += WAVES) {
-    int page = table[(size_t)b * W + p];
+  const int p0 = (int)((long long)npages * sh.part / ns), p1 = (int)((long long)npages * (sh.part + 1) / ns);
+  int ids = 0;                                    // lane i: the wave's i-th page from here on, and its scales
+  float kss = 0.f, vss = 0.f;
+  for (int p = p0 + w, turn = 0; p < p1; p += WAVES, ++turn) {
+    if ((turn & 63) == 0) {
+      ids = table[(size_t)b * W + min(p + lane * WAVES, npages - 1)];
+      const size_t at = (size_t)(ids < 0 || ids >= pages ? 0 : ids) * Hkv + hk;
+      kss = kscale[at];
+      vss = vscale[at];
+    }
+    int page = __builtin_amdgcn_readlane(ids, turn & 63);
+    const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), turn & 63));
+    const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vss), turn & 63));
     const bool bad = page < 0 || page >= pages;   // its keys count as masked
     page = bad ? 0 : page;
     const size_t ph = (size_t)page * Hkv + hk;
     const uint8_t* kp = kc + ph * PAGE * D;
     const uint8_t* vp = vc + ph * PAGE * D;
-    const float ks = kscale[ph], vs = vscale[ph];
-
     f32x4_t s[4];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
@@ -225,8 +257,8 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
 #pragma unroll
   for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4_t*>(&s_o[w][r][16 * i + 4 * a]) = o[i];
   __syncthreads();
-  const size_t slot0 = (size_t)first * Hkv + hk, slot_step = Hkv;     // the tile's parts in the workspace
-  const size_t slot = slot0 + s_part * slot_step;
+  const size_t slot0 = (size_t)(blockIdx.x - sh.part) * Hkv + hk, slot_step = Hkv;     // the tile's parts in the workspace
+  const size_t slot = slot0 + sh.part * slot_step;
   for (int x = t; x < TILE * (D / 4); x += NT) {
     const int rr = x / (D / 4), d = x % (D / 4) * 4;
     if (row0 + rr >= rows) continue;
@@ -257,26 +289,67 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
   // writes back the whole of the XCD's L2 for every part: 110 us against 20 for 32 rows of 1024 keys.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (t == 0) s_tile = __hip_atomic_fetch_add(&counters[slot0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (t == 0) s_last = __hip_atomic_fetch_add(&counters[slot0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ns - 1;
   __syncthreads();
-  if (s_tile != ns - 1) return;
+  if (!s_last) return;
   if (t == 0) __hip_atomic_store(&counters[slot0], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  for (int x = t; x < TILE * (D / 4); x += NT) {
-    const int rr = x / (D / 4), d = x % (D / 4) * 4;
-    if (row0 + rr >= rows) continue;
+  const int live = min(TILE, rows - row0);
+  float2* ml = reinterpret_cast<float2*>(s_raw);                      // [part][row]
+  float* joined = reinterpret_cast<float*>(s_raw + MAX_PARTS * TILE * 8);   // [thread][4 values, l]
+  for (int x = t; x < ns * live; x += NT) {
+    const int i = x / live, rr = x % live;
+    ml[i * TILE + rr] = get2(part_ml + ((slot0 + i * slot_step) * TILE + rr) * 2);
+  }
+  __syncthreads();
+  // four values a thread; few rows leave threads over, and each of `groups` takes every groups-th part
+  const int units = live * (D / 4), groups = max(NT / units, 1);
+  for (int x = t; x < units * groups; x += NT) {
+    const int unit = x % units, group = x / units, rr = unit / (D / 4), d = unit % (D / 4) * 4;
     float mm = -INFINITY;
-    for (int i = 0; i < ns; ++i) mm = fmaxf(mm, get2(part_ml + ((slot0 + i * slot_step) * TILE + rr) * 2).x);
+    for (int i = 0; i < ns; ++i) mm = fmaxf(mm, ml[i * TILE + rr].x);
     const float base = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f;
     f32x4_t oo = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < ns; ++i) {
-      const size_t at = (slot0 + i * slot_step) * TILE + rr;
-      const float2 ml = get2(part_ml + at * 2), x01 = get2(part_o + at * D + d), x23 = get2(part_o + at * D + d + 2);
-      const float f = __builtin_amdgcn_exp2f(ml.x - base);
-      ll += ml.y * f;
-      oo += f32x4_t{x01.x, x01.y, x23.x, x23.y} * f;
+    const float* at = part_o + (slot0 * TILE + rr) * D + d;
+    constexpr int AHEAD = 8;                      // loads in flight
+    for (int i0 = group; i0 < ns; i0 += groups * AHEAD) {
+      float2 x01[AHEAD], x23[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const float* src = at + (size_t)min(i0 + j * groups, ns - 1) * slot_step * TILE * D;
+        x01[j] = get2(src);
+        x23[j] = get2(src + 2);
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int i = i0 + j * groups;
+        if (i < ns) {
+          const float2 e = ml[i * TILE + rr];
+          const float f = __builtin_amdgcn_exp2f(e.x - base);
+          ll += e.y * f;
+          oo += f32x4_t{x01[j].x, x01[j].y, x23[j].x, x23[j].y} * f;
+        }
+      }
     }
-    store_row(out, oo, ll, row0 + rr, tok0, G, Hq, hk, D, d);
+    if (groups == 1) {
+      store_row(out, oo, ll, row0 + rr, tok0, G, Hq, hk, D, d);
+    } else {                                      // units * groups <= NT: one turn
+#pragma unroll
+      for (int j = 0; j < 4; ++j) joined[x * 5 + j] = oo[j];
+      joined[x * 5 + 4] = ll;
+    }
+  }
+  if (groups == 1) return;
+  __syncthreads();
+  if (t < units) {
+    float ll = 0.f;
+    f32x4_t oo = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < groups; ++g) {
+      const float* from = joined + (g * units + t) * 5;
+      oo += f32x4_t{from[0], from[1], from[2], from[3]};
+      ll += from[4];
+    }
+    store_row(out, oo, ll, row0 + t / (D / 4), tok0, G, Hq, hk, D, t % (D / 4) * 4);
   }
 }
 
