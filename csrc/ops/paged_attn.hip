@@ -69,64 +69,74 @@ struct Share {
   int b, tile, part, ns;     // ns: parts of the tile; 0: nothing left for this workgroup
 };
 
+// inclusive sum over the wave's lanes, without LDS (row shifts, then the rows' ends broadcast)
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
 // Every wave scans all requests by itself (contiguous ones in a lane): no barrier, and one round of loads for up to
-// 64 requests.
+// 64 requests.  The caller sees to it that the sums fit 31 bits.
 __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const int* __restrict__ kv_lens, int N, int B, int W,
                                             int G, int target) {
   const int lane = threadIdx.x & 63, per = (B + 63) / 64;
-  auto size = [&](int b, int* tiles, int* np) {
-    *tiles = *np = 0;
+  int tiles = 0, np = 0;
+  auto size = [&](int b) {
+    tiles = np = 0;
     if (b < B) {
       const int n = max(min(cu[b + 1], N) - min(max(cu[b], 0), N), 0);
-      *tiles = (n * G + TILE - 1) / TILE;
-      *np = (min(max(kv_lens[b], 0), W * PAGE) + PAGE - 1) / PAGE;
+      tiles = (n * G + TILE - 1) / TILE;
+      np = (min(max(kv_lens[b], 0), W * PAGE) + PAGE - 1) / PAGE;
     }
   };
-  int tiles, np;
-  long long sum = 0;
+  int sum = 0;
   for (int i = 0; i < per; ++i) {
-    size(lane * per + i, &tiles, &np);
-    sum += (long long)tiles * np;
+    size(lane * per + i);
+    sum += tiles * np;
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  const int chunk = (int)max((sum + target - 1) / target, (long long)MIN_CHUNK);
-  auto parts = [&](int np) { return min(max((np + chunk - 1) / chunk, 1), MAX_PARTS); };
-  sum = 0;
-  for (int i = 0; i < per; ++i) {
-    size(lane * per + i, &tiles, &np);
-    sum += (long long)tiles * parts(np);
+  const int all = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+  const int chunk = max((all + target - 1) / target, MIN_CHUNK);
+  auto parts = [&](int pages) { return min(max((pages + chunk - 1) / chunk, 1), MAX_PARTS); };
+  if (per == 1) {
+    sum = tiles * parts(np);
+  } else {
+    sum = 0;
+    for (int i = 0; i < per; ++i) {
+      size(lane * per + i);
+      sum += tiles * parts(np);
+    }
   }
-  long long at = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long u = __shfl_up(at, o, 64);
-    if (lane >= o) at += u;
-  }
-  at -= sum;
-  const unsigned long long owner = __ballot((long long)blockIdx.x >= at && (long long)blockIdx.x < at + sum);
+  const int end = wave_scan(sum), at = end - sum, me = (int)blockIdx.x;
+  const unsigned long long owner = __ballot(me >= at && me < end);
   Share sh = {0, 0, 0, 0};
   if (owner == 0) return sh;
   const int who = __ffsll((long long)owner) - 1;
-  int x = (int)(blockIdx.x - __shfl(at, who, 64));
-  for (int i = 0; i < per; ++i) {
-    size(who * per + i, &tiles, &np);
-    const int ns = parts(np);
-    if ((long long)x < (long long)tiles * ns) {
-      sh.b = who * per + i, sh.tile = x / ns, sh.part = x % ns, sh.ns = ns;
-      break;
+  int x = me - __builtin_amdgcn_readlane(at, who);
+  sh.b = who * per;
+  if (per == 1) {
+    sh.ns = __builtin_amdgcn_readlane(parts(np), who);
+  } else {
+    for (;; ++sh.b) {          // ends inside the lane's requests: x is below their sum
+      size(sh.b);
+      sh.ns = parts(np);
+      if (x < tiles * sh.ns) break;
+      x -= tiles * sh.ns;
     }
-    x -= tiles * ns;
   }
   sh.b = __builtin_amdgcn_readfirstlane(sh.b);
-  sh.tile = __builtin_amdgcn_readfirstlane(sh.tile);
-  sh.part = __builtin_amdgcn_readfirstlane(sh.part);
   sh.ns = __builtin_amdgcn_readfirstlane(sh.ns);
+  sh.tile = __builtin_amdgcn_readfirstlane(x / sh.ns);
+  sh.part = __builtin_amdgcn_readfirstlane(x % sh.ns);
   return sh;
 }
 
 template <int D>
-__global__ void __launch_bounds__(NT, 3)
+__global__ void __launch_bounds__(NT, 2)
 attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
             const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ table,
             const int* __restrict__ cu, const int* __restrict__ kv_lens, bf16_t* __restrict__ out,
@@ -174,39 +184,70 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
 
   const int npages = (most + PAGE - 1) / PAGE;
   const int p0 = (int)((long long)npages * sh.part / ns), p1 = (int)((long long)npages * (sh.part + 1) / ns);
-  int ids = 0;                                    // lane i: the wave's i-th page from here on, and its scales
+  const int turns = p1 - p0 > w ? (p1 - p0 - w + WAVES - 1) / WAVES : 0;   // pages of this wave
+  int ids = 0;                                    // lane i: one of the wave's next 64 pages, and its scales
   float kss = 0.f, vss = 0.f;
-  for (int p = p0 + w, turn = 0; p < p1; p += WAVES, ++turn) {
+  uint4 kr[4][KU], vr[DT];
+  struct Page {
+    size_t ph;
+    float ks, vs;
+    bool bad;                                     // not a page of the cache: its keys count as masked
+  };
+  auto page_at = [&](int turn) {
     if ((turn & 63) == 0) {
-      ids = table[(size_t)b * W + min(p + lane * WAVES, npages - 1)];
+      ids = table[(size_t)b * W + min(p0 + w + (turn + lane) * WAVES, npages - 1)];
       const size_t at = (size_t)(ids < 0 || ids >= pages ? 0 : ids) * Hkv + hk;
       kss = kscale[at];
       vss = vscale[at];
     }
-    int page = __builtin_amdgcn_readlane(ids, turn & 63);
-    const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), turn & 63));
-    const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vss), turn & 63));
-    const bool bad = page < 0 || page >= pages;   // its keys count as masked
-    page = bad ? 0 : page;
-    const size_t ph = (size_t)page * Hkv + hk;
-    const uint8_t* kp = kc + ph * PAGE * D;
-    const uint8_t* vp = vc + ph * PAGE * D;
+    const int id = __builtin_amdgcn_readlane(ids, turn & 63);
+    Page x;
+    x.ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), turn & 63));
+    x.vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vss), turn & 63));
+    x.bad = id < 0 || id >= pages;
+    x.ph = (size_t)(x.bad ? 0 : id) * Hkv + hk;
+    return x;
+  };
+  auto load_k = [&](size_t ph) {
+    const uint8_t* kp = kc + ph * PAGE * D + (size_t)(16 * (r >> 2) + (r & 3)) * D + 16 * a;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int u = 0; u < KU; ++u) kr[tt][u] = *reinterpret_cast<const uint4*>(kp + 4 * tt * D + 64 * u);
+  };
+  auto load_v = [&](size_t ph) {
+    const uint8_t* vp = vc + ph * PAGE * D + (size_t)r * PAGE + 16 * a;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) vr[i] = *reinterpret_cast<const uint4*>(vp + 16 * i * PAGE);
+  };
+  // K and V of a page are in registers before their turn: the next page's K is on its way from the moment that the
+  // scores have read this one's, its V from the moment that the output has
+  Page cur{}, next{};
+  if (turns > 0) {
+    cur = page_at(0);
+    load_k(cur.ph);
+    load_v(cur.ph);
+  }
+  for (int turn = 0; turn < turns; ++turn) {
     f32x4_t s[4];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
       s[tt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      const uint8_t* kr = kp + (size_t)(16 * (r >> 2) + 4 * tt + (r & 3)) * D;
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
-        const uint4 c = *reinterpret_cast<const uint4*>(kr + 16 * (a + 4 * u));
-        s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.x, c.y, ks), qf[u][0], s[tt], 0, 0, 0);
-        s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.z, c.w, ks), qf[u][1], s[tt], 0, 0, 0);
+        const uint4 c = kr[tt][u];
+        s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.x, c.y, cur.ks), qf[u][0], s[tt], 0, 0, 0);
+        s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.z, c.w, cur.ks), qf[u][1], s[tt], 0, 0, 0);
       }
     }
-    const int key0 = p * PAGE;
-    const int live = bad ? 0 : L - key0;          // keys of the page that were written
-    if (bad || key0 + PAGE > least) {
-      const int seen = bad ? 0 : vis - key0;
+    if (turn + 1 < turns) {
+      next = page_at(turn + 1);
+      load_k(next.ph);
+    }
+    const int key0 = (p0 + w + turn * WAVES) * PAGE;
+    const int live = cur.bad ? 0 : L - key0;      // keys of the page that were written
+    if (cur.bad || key0 + PAGE > least) {
+      const int seen = cur.bad ? 0 : vis - key0;
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
@@ -236,18 +277,20 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
         l += e;
         pf[h][j] = (__bf16)e;
       }
+    if (live < PAGE) {                            // slots never written may hold any code, NaN too
+      const uint32_t m0 = live_bytes(16 * a, live), m1 = live_bytes(16 * a + 4, live), m2 = live_bytes(16 * a + 8, live),
+                     m3 = live_bytes(16 * a + 12, live);
+#pragma unroll
+      for (int i = 0; i < DT; ++i) vr[i].x &= m0, vr[i].y &= m1, vr[i].z &= m2, vr[i].w &= m3;
+    }
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
-      uint4 c = *reinterpret_cast<const uint4*>(vp + (size_t)(16 * i + r) * PAGE + 16 * a);
-      if (live < PAGE) {                          // slots never written may hold any code, NaN too
-        c.x &= live_bytes(16 * a, live);
-        c.y &= live_bytes(16 * a + 4, live);
-        c.z &= live_bytes(16 * a + 8, live);
-        c.w &= live_bytes(16 * a + 12, live);
-      }
-      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.x, c.y, vs), pf[0], o[i], 0, 0, 0);
-      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.z, c.w, vs), pf[1], o[i], 0, 0, 0);
+      const uint4 c = vr[i];
+      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.x, c.y, cur.vs), pf[0], o[i], 0, 0, 0);
+      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.z, c.w, cur.vs), pf[1], o[i], 0, 0, 0);
     }
+    if (turn + 1 < turns) load_v(next.ph);
+    cur = next;
   }
 
   // join the waves
@@ -353,18 +396,9 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
   }
 }
 
-// No more tiles than this, whatever the lengths; parts: `target` more, as each part but a tile's last is a full chunk.
-long long most_tiles(long long N, int B, int G) { return N * G / TILE + (N < B ? N : B); }
-
 }  // namespace
 
 extern "C" {
-
-// Parts of a call (grid and workspace slots per kv head) for N tokens of B requests on a GPU of `cus` CUs.
-static long long most_parts(long long N, int B, int G, int Hkv, int cus, int* target) {
-  *target = (4 * cus + Hkv - 1) / Hkv;     // four workgroups fit a CU
-  return most_tiles(N, B, G) + *target;
-}
 
 int mivgpu_ops_visible_cus();
 static int all_cus() {
@@ -372,13 +406,25 @@ static int all_cus() {
   return n;
 }
 
-// counters (ints, zero before the first call, left zero), then (m, l) and O of the parts; in floats
-long long mivgpu_paged_attention_work(int N, int B, int Hq, int Hkv, int head_dim, long long* zeroed) {
+// Parts of a call (grid and workspace slots per kv head) for N tokens of B requests with tables of W pages: the tiles,
+// whatever the lengths, and `target` more, as each part but a tile's last is a full chunk; no more than all chunks.
+// target: two workgroups for each CU, all resident at once.
+static long long most_parts(long long N, int B, int G, int Hkv, long long W, int* target) {
+  *target = (2 * all_cus() + Hkv - 1) / Hkv;
+  const long long tiles = N * G / TILE + (N < B ? N : B), chunks = (W + MIN_CHUNK - 1) / MIN_CHUNK;
+  return chunks < (tiles + *target) / (tiles > 0 ? tiles : 1) ? tiles * chunks : tiles + *target;
+}
+
+// The workspace, for any head size: slots of a counter each (zero before the first call, left zero), then a tile's
+// (m, l) and O for each slot.  How it is divided follows from its size alone, so that calls of different sizes agree
+// on where the counters end.
+constexpr int SLOT_FLOATS = 1 + TILE * (2 + 128);
+
+long long mivgpu_paged_attention_work(int N, int B, int Hq, int Hkv, long long* zeroed) {
   if (N < 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return -1;
   int target;
-  const long long parts = most_parts(N, B, Hq / Hkv, Hkv, all_cus(), &target) * Hkv;
-  *zeroed = (parts + 3) / 4 * 4;
-  return *zeroed + parts * TILE * (2 + head_dim);
+  *zeroed = (most_parts(N, B, Hq / Hkv, Hkv, INT_MAX, &target) * Hkv + 3) / 4 * 4;
+  return *zeroed * SLOT_FLOATS;
 }
 
 int mivgpu_paged_attention(const void* q, const void* kc, const void* vc, const float* kscale, const float* vscale,
@@ -389,14 +435,13 @@ int mivgpu_paged_attention(const void* q, const void* kc, const void* vc, const 
     return -1;
   if (N == 0) return 0;
   const int G = Hq / Hkv;
-  long long zeroed;
-  const long long need = mivgpu_paged_attention_work(N, B, Hq, Hkv, head_dim, &zeroed);
-  if (work == nullptr || floats < need) return -2;
   int target;
-  const long long parts = most_parts(N, B, G, Hkv, all_cus(), &target);
-  if (parts > INT_MAX) return -1;
-  float* ml = work + zeroed;
-  float* po = ml + parts * Hkv * TILE * 2;
+  const long long parts = most_parts(N, B, G, Hkv, W, &target);
+  if (parts * W > INT_MAX) return -1;
+  const long long slots = floats / SLOT_FLOATS / 4 * 4;
+  if (work == nullptr || slots < parts * Hkv) return -2;
+  float* ml = work + slots;
+  float* po = ml + slots * TILE * 2;
   const dim3 grid((unsigned)parts, Hkv);
   const float sl2 = scale * 1.4426950408889634f;
 #define MIVGPU_PATTN(DD)                                                                                              \

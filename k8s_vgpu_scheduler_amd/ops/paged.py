@@ -235,7 +235,7 @@ def paged_attention_workspace(n_tokens: int, rows: int, n_q_heads: int, n_kv_hea
                          f"heads of {head_dim} (64 or 128)")
     zeroed = ctypes.c_longlong(0)
     with torch.cuda.device(device):
-        floats = ops.lib().mivgpu_paged_attention_work(n_tokens, rows, n_q_heads, n_kv_heads, head_dim, ctypes.byref(zeroed))
+        floats = ops.lib().mivgpu_paged_attention_work(n_tokens, rows, n_q_heads, n_kv_heads, ctypes.byref(zeroed))
     work = torch.empty(floats, dtype=_F32, device=device)
     work[:zeroed.value].zero_()
     return work
