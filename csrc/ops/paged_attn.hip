@@ -5,12 +5,15 @@
 //   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale (q_i . k_j) - m_i)
 // in one pass over the pages with the running maximum m and sum (fp32).
 //
-// The rows of one kv head's G query heads are flattened (row = token * G + head) and cut into tiles of 16.  A tile's
-// pages are split over as many workgroups as keep the chip evenly busy: every workgroup scans the requests' lengths
-// (at most 1024: a few a thread) and takes its share of all tiles' pages, so that one long request among short ones
-// is cut into more parts and nothing is planned on the host.  In a workgroup four waves take every fourth page and
-// join their (m, l, O) in LDS; the parts of a tile leave theirs in the workspace, and the last one to arrive (a
-// counter that it sets back to zero) joins them in the order of the parts.  Per page of 64 keys a wave
+// The rows of one kv head's G query heads are flattened (row = token * G + head) and cut into tiles: of 16 rows where
+// a request brings at most SHORT_ROWS of them (decode, a few tokens), of 256 in the others (chunks, prompts); a kernel
+// for each kind.  A tile's pages are split over as many workgroups as keep the chip evenly busy: every workgroup scans
+// the requests' lengths (at most 1024: a few a lane) and takes its share of all tiles' pages, so that one long request
+// among short ones is cut into more parts and nothing is planned on the host.  The parts of a tile leave their
+// (m, l, O) in the workspace, and the last one to arrive (a counter that it sets back to zero) joins them in the order
+// of the parts, so that a call's bits do not depend on who that is.
+//
+// Tiles of 16: the four waves of a workgroup take every fourth page and join in LDS.  Per page of 64 keys a wave
 // computes, with 16x16x32 bf16 MFMAs,
 //   S^T (64 keys x 16 rows) = K . Q^T        4 tiles of 16 keys: tile t's row 4a + c is key 16a + 4t + c, so that
 //                                            lane (row r, quarter a) ends with the 16 consecutive keys 16a .. 16a+15;
@@ -28,9 +31,22 @@ typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+
+// short requests
 constexpr int NT = 256, WAVES = 4, TILE = 16;
 constexpr int MIN_CHUNK = WAVES;         // pages of a part: at least one for each wave
 constexpr int MAX_PARTS = 256;           // of a tile: their (m, l) take 32 KB of LDS
+constexpr int SHORT_ROWS = 64;
+// long requests
+constexpr int LNT = 512, LWAVES = 8, LTILE = 32 * LWAVES;
+constexpr int LMIN_CHUNK = 8;
+
+// Workgroups that a call aims at (two a CU, one a CU), over all kv heads, and with them the slots of the workspace.
+// With t parts aimed at a kv head a split tile of np pages gets at most np / chunk + 1 <= 2 np / chunk parts, which
+// add up to at most 2 t.
+constexpr int MAX_CUS = 256, MAX_HKV = 256;
+constexpr int SHORT_SLOTS = 2 * 2 * MAX_CUS, LONG_SLOTS = 2 * MAX_CUS;
 
 // 8 codes -> 8 bf16, times 2^e
 __device__ __forceinline__ bf16x8_t widen(uint32_t lo, uint32_t hi, float s) {
@@ -67,6 +83,7 @@ __device__ __forceinline__ void store_row(bf16_t* out, f32x4_t o, float l, int r
 // which request, tile of its rows and part of that tile's pages a workgroup takes, from its index among all parts
 struct Share {
   int b, tile, part, ns;     // ns: parts of the tile; 0: nothing left for this workgroup
+  int slot;                  // of the tile's first part, among the split tiles' parts
 };
 
 // inclusive sum over the wave's lanes, without LDS (row shifts, then the rows' ends broadcast)
@@ -80,18 +97,23 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// Every wave scans all requests by itself (contiguous ones in a lane): no barrier, and one round of loads for up to
-// 64 requests.  The caller sees to it that the sums fit 31 bits.
+// Every wave scans all requests of more than `above` and at most `upto` rows by itself (contiguous ones in a lane): no
+// barrier, and one round of loads for up to 64 requests.  Workgroup 0 takes the last part of all: in a prompt the
+// tiles at the end have the most keys, and the longest work should start first.  The caller sees to it that the sums
+// fit 31 bits.
+template <int ROWS, int SMALLEST>
 __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const int* __restrict__ kv_lens, int N, int B, int W,
-                                            int G, int target) {
+                                            int G, int target, int above, int upto, int me) {
   const int lane = threadIdx.x & 63, per = (B + 63) / 64;
   int tiles = 0, np = 0;
   auto size = [&](int b) {
     tiles = np = 0;
     if (b < B) {
-      const int n = max(min(cu[b + 1], N) - min(max(cu[b], 0), N), 0);
-      tiles = (n * G + TILE - 1) / TILE;
-      np = (min(max(kv_lens[b], 0), W * PAGE) + PAGE - 1) / PAGE;
+      const int rows = max(min(cu[b + 1], N) - min(max(cu[b], 0), N), 0) * G;
+      if (rows > above && rows <= upto) {
+        tiles = (rows + ROWS - 1) / ROWS;
+        np = (min(max(kv_lens[b], 0), W * PAGE) + PAGE - 1) / PAGE;
+      }
     }
   };
   int sum = 0;
@@ -99,25 +121,26 @@ __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const in
     size(lane * per + i);
     sum += tiles * np;
   }
-  const int all = __builtin_amdgcn_readlane(wave_scan(sum), 63);
-  const int chunk = max((all + target - 1) / target, MIN_CHUNK);
+  const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+  const int chunk = max((total + target - 1) / target, SMALLEST);
   auto parts = [&](int pages) { return min(max((pages + chunk - 1) / chunk, 1), MAX_PARTS); };
-  if (per == 1) {
-    sum = tiles * parts(np);
-  } else {
-    sum = 0;
-    for (int i = 0; i < per; ++i) {
-      size(lane * per + i);
-      sum += tiles * parts(np);
-    }
+  int split = 0;
+  sum = 0;
+  for (int i = 0; i < per; ++i) {
+    if (per > 1) size(lane * per + i);
+    const int ns = parts(np);
+    sum += tiles * ns;
+    split += ns > 1 ? tiles * ns : 0;
   }
-  const int end = wave_scan(sum), at = end - sum, me = (int)blockIdx.x;
+  const int end = wave_scan(sum), at = end - sum, slot = wave_scan(split) - split;
+  me = __builtin_amdgcn_readlane(end, 63) - 1 - me;
   const unsigned long long owner = __ballot(me >= at && me < end);
-  Share sh = {0, 0, 0, 0};
+  Share sh = {0, 0, 0, 0, 0};
   if (owner == 0) return sh;
   const int who = __ffsll((long long)owner) - 1;
   int x = me - __builtin_amdgcn_readlane(at, who);
   sh.b = who * per;
+  sh.slot = __builtin_amdgcn_readlane(slot, who);
   if (per == 1) {
     sh.ns = __builtin_amdgcn_readlane(parts(np), who);
   } else {
@@ -126,12 +149,14 @@ __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const in
       sh.ns = parts(np);
       if (x < tiles * sh.ns) break;
       x -= tiles * sh.ns;
+      sh.slot += sh.ns > 1 ? tiles * sh.ns : 0;
     }
   }
   sh.b = __builtin_amdgcn_readfirstlane(sh.b);
   sh.ns = __builtin_amdgcn_readfirstlane(sh.ns);
   sh.tile = __builtin_amdgcn_readfirstlane(x / sh.ns);
   sh.part = __builtin_amdgcn_readfirstlane(x % sh.ns);
+  sh.slot = __builtin_amdgcn_readfirstlane(sh.slot) + sh.tile * sh.ns;
   return sh;
 }
 
@@ -141,7 +166,7 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
             const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ table,
             const int* __restrict__ cu, const int* __restrict__ kv_lens, bf16_t* __restrict__ out,
             int* __restrict__ counters, float* __restrict__ part_ml, float* __restrict__ part_o, int N, int B, int W,
-            int Hq, int Hkv, int pages, int target, float scale_log2) {
+            int Hq, int Hkv, int pages, int target, int upto, float scale_log2) {
   constexpr int KU = D / 64;              // 16-byte chunks of a K row per lane
   constexpr int DT = D / 16;              // output tiles
   __shared__ float s_m[WAVES][TILE], s_l[WAVES][TILE];
@@ -153,7 +178,7 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 15, a = lane >> 4;
   const int G = Hq / Hkv, hk = blockIdx.y;
-  const Share sh = find_share(cu, kv_lens, N, B, W, G, target);
+  const Share sh = find_share<TILE, MIN_CHUNK>(cu, kv_lens, N, B, W, G, target, 0, upto, blockIdx.x);
   if (sh.ns == 0) return;
   const int b = sh.b, row0 = sh.tile * TILE, ns = sh.ns;
   const int tok0 = min(max(cu[b], 0), N), n = min(cu[b + 1], N) - tok0, rows = n * G;
@@ -300,7 +325,7 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
 #pragma unroll
   for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4_t*>(&s_o[w][r][16 * i + 4 * a]) = o[i];
   __syncthreads();
-  const size_t slot0 = (size_t)(blockIdx.x - sh.part) * Hkv + hk, slot_step = Hkv;     // the tile's parts in the workspace
+  const size_t slot0 = (size_t)sh.slot * Hkv + hk, slot_step = Hkv;     // the tile's parts in the workspace
   const size_t slot = slot0 + sh.part * slot_step;
   for (int x = t; x < TILE * (D / 4); x += NT) {
     const int rr = x / (D / 4), d = x % (D / 4) * 4;
@@ -396,6 +421,243 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
   }
 }
 
+// ------------------------------------------------------------------------------------------------ long requests --
+// Eight waves of 32 rows share every page: its codes become bf16 once, on their way from registers (a 16-byte load
+// of K and of V a thread, a page ahead) to LDS, double-buffered with one barrier a page.  Per page a wave computes,
+// with 32x32x16 bf16 MFMAs,
+//   S^T (2 x 32 keys x 32 rows) = K . Q^T     lane (row r, half h) holds the keys (i & 3) + 8 (i >> 2) + 4 h of each 32;
+//   O^T (D x 32 rows) += V^T . P^T            eight registers of S^T are the operand of a k-step of 16 keys: keys
+//                                             {0-3, 8-11} + 4 h; V's 16 keys are stored in two chunks in that order.
+// LDS rows are permuted by 16-byte chunks (chunk ^ row) so that the lanes of a read cover all banks.
+// The output and sum are rescaled only where a row's maximum grew by more than 8 (in log2): the p stay below 2^8,
+// which neither bf16 nor the sums mind.
+// Bound: the matrix instructions, with the exponentials beside them.
+template <int D>
+__device__ __forceinline__ int k_at(int row, int ch) { return row * D + ((ch ^ (row & (D / 8 - 1))) << 3); }
+__device__ __forceinline__ int v_at(int dim, int ch) { return dim * PAGE + ((ch ^ (dim & 7)) << 3); }
+
+template <int D>
+__global__ void __launch_bounds__(LNT, 2)
+attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+                 const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ table,
+                 const int* __restrict__ cu, const int* __restrict__ kv_lens, bf16_t* __restrict__ out,
+                 int* __restrict__ counters, float* __restrict__ part_ml, float* __restrict__ part_o, int N, int B, int W,
+                 int Hq, int Hkv, int pages, int target, float scale_log2) {
+  constexpr int KS = D / 16, DC = D / 32;              // k-steps of the scores, 32-wide blocks of the output
+  constexpr int CHUNKS = PAGE * D / 16;                // 16-byte chunks of codes in a page, each of K and V
+  __shared__ __attribute__((aligned(16))) bf16_t s_k[2][PAGE * D], s_v[2][PAGE * D];
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int r = lane & 31, h = lane >> 5;
+  // kv head = workgroup mod Hkv: with 8 of them each XCD's L2 serves one head's pages
+  const int G = Hq / Hkv, hk = blockIdx.x % Hkv;
+  const Share sh = find_share<LTILE, LMIN_CHUNK>(cu, kv_lens, N, B, W, G, target, SHORT_ROWS, INT_MAX, blockIdx.x / Hkv);
+  if (sh.ns == 0) return;
+  const int b = sh.b, ns = sh.ns, tile0 = sh.tile * LTILE, row0 = tile0 + 32 * w;
+  const int tok0 = min(max(cu[b], 0), N), n = min(cu[b + 1], N) - tok0, rows = n * G;
+  const int L = min(max(kv_lens[b], 0), W * PAGE);
+  const int row = min(row0 + r, rows - 1);             // rows behind the last repeat it
+  const int vis = max(L - n + row / G + 1, 0);
+  const int least = max(L - n + min(row0, rows - 1) / G + 1, 0), most = max(L - n + min(row0 + 31, rows - 1) / G + 1, 0);
+  const int tile_most = max(L - n + min(tile0 + LTILE - 1, rows - 1) / G + 1, 0);
+  const bool idle = row0 >= rows;
+
+  bf16x8_t qf[KS];
+  {
+    const bf16_t* qp = q + ((size_t)(tok0 + row / G) * Hq + (size_t)hk * G + row % G) * D + 8 * h;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * s);
+  }
+  f32x16_t o[DC];
+#pragma unroll
+  for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dc][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  const int npages = (min(tile_most, L) + PAGE - 1) / PAGE;
+  const int p0 = (int)((long long)npages * sh.part / ns), p1 = (int)((long long)npages * (sh.part + 1) / ns);
+  int ids = 0;                                         // lane i: one of the next 64 pages, and its scales
+  float kss = 0.f, vss = 0.f;
+  uint4 kr = make_uint4(0, 0, 0, 0), vr = kr;          // the next page's codes, and what goes with them
+  float ks = 0.f, vs = 0.f;
+  bool bad = false;
+  auto fetch = [&](int p) {
+    const int at = (p - p0) & 63;
+    if (at == 0) {
+      ids = table[(size_t)b * W + min(p + lane, npages - 1)];
+      const size_t x = (size_t)(ids < 0 || ids >= pages ? 0 : ids) * Hkv + hk;
+      kss = kscale[x];
+      vss = vscale[x];
+    }
+    const int id = __builtin_amdgcn_readlane(ids, at);
+    ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), at));
+    vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vss), at));
+    bad = id < 0 || id >= pages;
+    const size_t ph = ((size_t)(bad ? 0 : id) * Hkv + hk) * (PAGE * D);
+    if (t < CHUNKS) {
+      kr = *reinterpret_cast<const uint4*>(kc + ph + 16 * t);
+      vr = *reinterpret_cast<const uint4*>(vc + ph + 16 * t);
+    }
+  };
+  auto stage = [&](int buf, int p) {
+    if (t < CHUNKS) {
+      const int kt = t / (D / 16), kch = t % (D / 16) * 2;
+      *reinterpret_cast<bf16x8_t*>(&s_k[buf][k_at<D>(kt, kch)]) = widen(kr.x, kr.y, ks);
+      *reinterpret_cast<bf16x8_t*>(&s_k[buf][k_at<D>(kt, kch + 1)]) = widen(kr.z, kr.w, ks);
+      const int dim = t / (PAGE / 16), qk = t % (PAGE / 16), live = bad ? 0 : L - p * PAGE;
+      if (live < PAGE) {                               // slots never written may hold any code, NaN too
+        vr.x &= live_bytes(16 * qk, live);
+        vr.y &= live_bytes(16 * qk + 4, live);
+        vr.z &= live_bytes(16 * qk + 8, live);
+        vr.w &= live_bytes(16 * qk + 12, live);
+      }
+      *reinterpret_cast<bf16x8_t*>(&s_v[buf][v_at(dim, 2 * qk)]) = widen(vr.x, vr.z, vs);
+      *reinterpret_cast<bf16x8_t*>(&s_v[buf][v_at(dim, 2 * qk + 1)]) = widen(vr.y, vr.w, vs);
+    }
+  };
+
+  if (p0 < p1) {
+    fetch(p0);
+    stage(0, p0);
+  }
+  __syncthreads();
+  for (int p = p0; p < p1; ++p) {
+    const int buf = (p - p0) & 1, key0 = p * PAGE;
+    const bool masked = bad;                           // of this page; fetch moves on to the next
+    if (p + 1 < p1) fetch(p + 1);
+    if (!idle && key0 < most) {
+      const bool two = key0 + 32 < most;               // some row sees a key of the second half
+      const bf16_t* sk = s_k[buf];
+      const bf16_t* sv = s_v[buf];
+      f32x16_t s0, s1;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s0[i] = 0.f, s1[i] = 0.f;
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+        s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(&sk[k_at<D>(r, 2 * st + h)]), qf[st], s0, 0, 0, 0);
+      if (two) {
+#pragma unroll
+        for (int st = 0; st < KS; ++st)
+          s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(&sk[k_at<D>(32 + r, 2 * st + h)]), qf[st], s1, 0, 0, 0);
+      }
+      if (masked || key0 + PAGE > least) {
+        const int seen = (masked ? 0 : vis - key0) - 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if ((i & 3) + 8 * (i >> 2) >= seen) s0[i] = -INFINITY;
+          if ((i & 3) + 8 * (i >> 2) + 32 >= seen) s1[i] = -INFINITY;
+        }
+      }
+      float mx = s0[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s0[i]);
+      if (two) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s1[i]);
+      }
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mt = mx * scale_log2;
+      if (__ballot(mt > m + 8.f)) {
+        const float mnew = fmaxf(m, mt);
+        const float alpha = __builtin_amdgcn_exp2f(m - (mnew == -INFINITY ? 0.f : mnew));
+        m = mnew;
+        l *= alpha;
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[dc][i] *= alpha;
+      }
+      const float base = m == -INFINITY ? 0.f : m;     // nothing seen yet: every p is exp2(-inf) = 0
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s0[i] = __builtin_amdgcn_exp2f(fmaf(s0[i], scale_log2, -base));
+        sum += s0[i];
+      }
+      if (two) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s1[i] = __builtin_amdgcn_exp2f(fmaf(s1[i], scale_log2, -base));
+          sum += s1[i];
+        }
+      }
+      l += sum;
+      auto pv = [&](const f32x16_t& s, int u) {        // k-step u of the page's four
+        bf16x8_t pf;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[8 * (u & 1) + j];
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc)
+          o[dc] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(&sv[v_at(32 * dc + r, 2 * u + h)]), pf, o[dc], 0, 0, 0);
+      };
+      pv(s0, 0);
+      pv(s0, 1);
+      if (two) {
+        pv(s1, 2);
+        pv(s1, 3);
+      }
+    }
+    if (p + 1 < p1) stage(buf ^ 1, p + 1);
+    __syncthreads();
+  }
+
+  // lane (r, h) holds dims 32 dc + 8 j + 4 h .. + 4 of its row
+  l += __shfl_xor(l, 32, 64);
+  const size_t slot0 = (size_t)sh.slot * Hkv + hk, mine = (slot0 + (size_t)sh.part * Hkv) * LTILE + 32 * w + r;
+  if (row0 + r < rows) {
+#pragma unroll
+    for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = 32 * dc + 8 * j + 4 * h;
+        const f32x4_t x = {o[dc][4 * j], o[dc][4 * j + 1], o[dc][4 * j + 2], o[dc][4 * j + 3]};
+        if (ns == 1) {
+          store_row(out, x, l, row, tok0, G, Hq, hk, D, d);
+        } else {
+          put2(part_o + mine * D + d, x[0], x[1]);
+          put2(part_o + mine * D + d + 2, x[2], x[3]);
+        }
+      }
+    if (ns > 1 && h == 0) put2(part_ml + mine * 2, m, l);
+  }
+  if (ns == 1) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // as in attn_kernel
+  __syncthreads();
+  int* s_last = reinterpret_cast<int*>(s_k);
+  if (t == 0) *s_last = __hip_atomic_fetch_add(&counters[slot0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ns - 1;
+  __syncthreads();
+  if (!*s_last) return;
+  if (t == 0) __hip_atomic_store(&counters[slot0], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const int live = min(LTILE, rows - tile0);
+  for (int x = t; x < live * (D / 4); x += LNT) {
+    const int rr = x / (D / 4), d = x % (D / 4) * 4;
+    float mm = -INFINITY, ll = 0.f;
+    f32x4_t oo = {0.f, 0.f, 0.f, 0.f};
+    constexpr int AHEAD = 4;                           // loads in flight
+    for (int i0 = 0; i0 < ns; i0 += AHEAD) {
+      float2 ml[AHEAD], x01[AHEAD], x23[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const size_t at = (slot0 + (size_t)min(i0 + j, ns - 1) * Hkv) * LTILE + rr;
+        ml[j] = get2(part_ml + at * 2);
+        x01[j] = get2(part_o + at * D + d);
+        x23[j] = get2(part_o + at * D + d + 2);
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (i0 + j < ns) {
+          const float mnew = fmaxf(mm, ml[j].x), base = mnew == -INFINITY ? 0.f : mnew;
+          const float f0 = __builtin_amdgcn_exp2f(mm - base), f1 = __builtin_amdgcn_exp2f(ml[j].x - base);
+          mm = mnew;
+          ll = ll * f0 + ml[j].y * f1;
+          oo = oo * f0 + f32x4_t{x01[j].x, x01[j].y, x23[j].x, x23[j].y} * f1;
+        }
+      }
+    }
+    store_row(out, oo, ll, tile0 + rr, tok0, G, Hq, hk, D, d);
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -403,54 +665,66 @@ extern "C" {
 int mivgpu_ops_visible_cus();
 static int all_cus() {
   static const int n = mivgpu_ops_visible_cus();
-  return n;
+  return n < MAX_CUS ? n : MAX_CUS;
 }
 
-// Parts of a call (grid and workspace slots per kv head) for N tokens of B requests with tables of W pages: the tiles,
-// whatever the lengths, and `target` more, as each part but a tile's last is a full chunk; no more than all chunks.
-// target: two workgroups for each CU, all resident at once.
-static long long most_parts(long long N, int B, int G, int Hkv, long long W, int* target) {
-  *target = (2 * all_cus() + Hkv - 1) / Hkv;
-  const long long tiles = N * G / TILE + (N < B ? N : B), chunks = (W + MIN_CHUNK - 1) / MIN_CHUNK;
-  return chunks < (tiles + *target) / (tiles > 0 ? tiles : 1) ? tiles * chunks : tiles + *target;
+// The workspace, for any head size: counters (zero before the first call, left zero), then (m, l) and O of the short
+// and, where a call has more rows than SHORT_ROWS, of the long tiles' parts.
+constexpr long long ZEROED = SHORT_SLOTS + LONG_SLOTS;
+constexpr long long SHORT_FLOATS = (long long)SHORT_SLOTS * TILE * (2 + 128);
+constexpr long long LONG_FLOATS = (long long)LONG_SLOTS * LTILE * (2 + 128);
+
+long long mivgpu_paged_attention_work(int N, int Hq, int Hkv, long long* zeroed) {
+  if (N < 0 || Hq <= 0 || Hkv <= 0 || Hkv > MAX_HKV || Hq % Hkv) return -1;
+  *zeroed = ZEROED;
+  return ZEROED + SHORT_FLOATS + ((long long)N * (Hq / Hkv) > SHORT_ROWS ? LONG_FLOATS : 0);
 }
 
-// The workspace, for any head size: slots of a counter each (zero before the first call, left zero), then a tile's
-// (m, l) and O for each slot.  How it is divided follows from its size alone, so that calls of different sizes agree
-// on where the counters end.
-constexpr int SLOT_FLOATS = 1 + TILE * (2 + 128);
-
-long long mivgpu_paged_attention_work(int N, int B, int Hq, int Hkv, long long* zeroed) {
-  if (N < 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return -1;
-  int target;
-  *zeroed = (most_parts(N, B, Hq / Hkv, Hkv, INT_MAX, &target) * Hkv + 3) / 4 * 4;
-  return *zeroed * SLOT_FLOATS;
-}
-
+// max_new: the most new tokens of a request, or negative if not known
 int mivgpu_paged_attention(const void* q, const void* kc, const void* vc, const float* kscale, const float* vscale,
                            const int* table, const int* cu, const int* kv_lens, void* out, float* work, long long floats,
-                           int N, int B, int W, int Hq, int Hkv, int head_dim, int pages, float scale, hipStream_t s) {
-  if (N < 0 || B <= 0 || B > MAX_ROWS || W <= 0 || (long long)W * PAGE > INT_MAX || Hq <= 0 || Hkv <= 0 || Hq % Hkv ||
-      Hkv > 65535 || pages <= 0 || (long long)N * (Hq / Hkv) > INT_MAX / 2)
+                           int N, int B, int W, int Hq, int Hkv, int head_dim, int pages, int max_new, float scale,
+                           hipStream_t s) {
+  if (N < 0 || B <= 0 || B > MAX_ROWS || W <= 0 || (long long)W * PAGE > INT_MAX || Hq <= 0 || Hkv <= 0 ||
+      Hkv > MAX_HKV || Hq % Hkv || pages <= 0 || (long long)N * (Hq / Hkv) > INT_MAX / 2 ||
+      (head_dim != 64 && head_dim != 128))
     return -1;
   if (N == 0) return 0;
   const int G = Hq / Hkv;
-  int target;
-  const long long parts = most_parts(N, B, G, Hkv, W, &target);
-  if (parts * W > INT_MAX) return -1;
-  const long long slots = floats / SLOT_FLOATS / 4 * 4;
-  if (work == nullptr || slots < parts * Hkv) return -2;
-  float* ml = work + slots;
-  float* po = ml + slots * TILE * 2;
-  const dim3 grid((unsigned)parts, Hkv);
+  const long long rows = (long long)N * G, some = N < B ? N : B;
+  // All rows through the short kernel where no request is long; then it also takes one that is longer than it was
+  // said to be.
+  const bool longs = rows > SHORT_ROWS && (max_new < 0 || (long long)max_new * G > SHORT_ROWS);
+  if (work == nullptr || floats < ZEROED + SHORT_FLOATS + (longs ? LONG_FLOATS : 0)) return -2;
+  float* sml = work + ZEROED;
+  float* so = sml + SHORT_SLOTS * TILE * 2;
+  float* lml = sml + SHORT_FLOATS;
+  float* lo = lml + LONG_SLOTS * LTILE * 2;
   const float sl2 = scale * 1.4426950408889634f;
+  // Parts: no more than the tiles there can be and `target` on top (each part but a tile's last is a whole chunk), nor
+  // than all chunks of all tiles
+  auto grid_of = [&](long long tiles, int target, int chunk) {
+    const long long all = tiles * ((W + chunk - 1) / chunk), most = tiles + target;
+    return all < most ? all : most;
+  };
+  const int target = 2 * all_cus() / Hkv > 1 ? 2 * all_cus() / Hkv : 1, ltarget = all_cus() / Hkv > 1 ? all_cus() / Hkv : 1;
+  long long tiles = rows / TILE + some;
+  if (longs && tiles > some * (SHORT_ROWS / TILE)) tiles = some * (SHORT_ROWS / TILE);
+  const long long few = rows / (SHORT_ROWS + 1), ltiles = rows / LTILE + (few < some ? few : some);
+  const long long parts = grid_of(tiles, target, MIN_CHUNK), lparts = grid_of(ltiles, ltarget, LMIN_CHUNK) * Hkv;
+  if (tiles * W > INT_MAX || (longs && ltiles * W > INT_MAX) || parts > INT_MAX || lparts > INT_MAX) return -1;
 #define MIVGPU_PATTN(DD)                                                                                              \
-  hipLaunchKernelGGL(attn_kernel<DD>, grid, dim3(NT), 0, s, (const bf16_t*)q, (const uint8_t*)kc, (const uint8_t*)vc, \
-                     kscale, vscale, table, cu, kv_lens, (bf16_t*)out, (int*)work, ml, po, N, B, W, Hq, Hkv, pages,   \
-                     target, sl2)
+  do {                                                                                                                \
+    if (longs)                                                                                                        \
+      hipLaunchKernelGGL(attn_long_kernel<DD>, dim3((unsigned)lparts), dim3(LNT), 0, s, (const bf16_t*)q,             \
+                         (const uint8_t*)kc, (const uint8_t*)vc, kscale, vscale, table, cu, kv_lens, (bf16_t*)out,    \
+                         (int*)work + SHORT_SLOTS, lml, lo, N, B, W, Hq, Hkv, pages, ltarget, sl2);                   \
+    hipLaunchKernelGGL(attn_kernel<DD>, dim3((unsigned)parts, Hkv), dim3(NT), 0, s, (const bf16_t*)q,                 \
+                       (const uint8_t*)kc, (const uint8_t*)vc, kscale, vscale, table, cu, kv_lens, (bf16_t*)out,      \
+                       (int*)work, sml, so, N, B, W, Hq, Hkv, pages, target, longs ? SHORT_ROWS : INT_MAX, sl2);      \
+  } while (0)
   if (head_dim == 128) MIVGPU_PATTN(128);
-  else if (head_dim == 64) MIVGPU_PATTN(64);
-  else return -1;
+  else MIVGPU_PATTN(64);
 #undef MIVGPU_PATTN
   return (int)hipGetLastError();
 }

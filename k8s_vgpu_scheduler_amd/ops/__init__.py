@@ -69,8 +69,8 @@ def lib():
         L.mivgpu_page_plan.argtypes = [vp] * 10 + [i] * 4 + [vp]
         L.mivgpu_page_commit.argtypes = [vp] * 7 + [i] * 3 + [vp]
         L.mivgpu_paged_qk_norm_rope_kv.argtypes = [vp, ll] + [vp] * 10 + [i] * 5 + [f, vp]
-        L.mivgpu_paged_attention.argtypes = [vp] * 10 + [ll] + [i] * 7 + [f, vp]
-        L.mivgpu_paged_attention_work.argtypes = [i] * 4 + [ctypes.POINTER(ll)]
+        L.mivgpu_paged_attention.argtypes = [vp] * 10 + [ll] + [i] * 8 + [f, vp]
+        L.mivgpu_paged_attention_work.argtypes = [i] * 3 + [ctypes.POINTER(ll)]
         L.mivgpu_paged_attention_work.restype = ll
         L.mivgpu_sample.argtypes = [vp, ll, i, i] + [vp] * 7 + [vp]
         for fn in ("mivgpu_rmsnorm", "mivgpu_add_rmsnorm", "mivgpu_qk_norm_rope_kv",

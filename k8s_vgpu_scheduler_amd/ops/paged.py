@@ -235,7 +235,7 @@ def paged_attention_workspace(n_tokens: int, rows: int, n_q_heads: int, n_kv_hea
                          f"heads of {head_dim} (64 or 128)")
     zeroed = ctypes.c_longlong(0)
     with torch.cuda.device(device):
-        floats = ops.lib().mivgpu_paged_attention_work(n_tokens, rows, n_q_heads, n_kv_heads, ctypes.byref(zeroed))
+        floats = ops.lib().mivgpu_paged_attention_work(n_tokens, n_q_heads, n_kv_heads, ctypes.byref(zeroed))
     work = torch.empty(floats, dtype=_F32, device=device)
     work[:zeroed.value].zero_()
     return work
@@ -269,5 +269,5 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, table: torch.Tensor, cu_q: 
         raise ValueError(f"{name}: work must be from paged_attention_workspace on {q.device}")
     _aligned(name, q=p[0], k=p[1], v=p[2], out=p[8], work=work.data_ptr())
     _launch(idx, name, ops.lib().mivgpu_paged_attention, *p, work.data_ptr(), work.numel(), N, B, W, n_q_heads, n_kv_heads,
-            head_dim, pages, scale)
+            head_dim, pages, -1 if max_new is None else max_new, scale)
     return out
