@@ -17,13 +17,11 @@ constexpr uint8_t CODE_NAN = 0x7f;
 
 __device__ __forceinline__ float bf2f(bf16_t x) { return __uint_as_float(((uint32_t)x) << 16); }
 
-// round to nearest even; NaN stays NaN
-__device__ __forceinline__ uint32_t f2bf(float f) {
-  uint32_t u = __float_as_uint(f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (u >> 16) | 0x40u;
-  return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+// two floats to bf16, round to nearest even, NaN stays NaN: one instruction
+__device__ __forceinline__ uint32_t pack2bf(float a, float b) {
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
+  return __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)a, (__bf16)b});
 }
-__device__ __forceinline__ uint32_t pack2bf(float a, float b) { return f2bf(a) | (f2bf(b) << 16); }
 
 __device__ __forceinline__ void unpack8(const uint4& v, float* f) {
   f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);

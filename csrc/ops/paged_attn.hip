@@ -431,6 +431,8 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
 // LDS rows are permuted by 16-byte chunks (chunk ^ row) so that the lanes of a read cover all banks.
 // The output and sum are rescaled only where a row's maximum grew by more than 8 (in log2): the p stay below 2^8,
 // which neither bf16 nor the sums mind.
+// Measured and left out (8192-token prompt, this kernel 565 us): the two waves of a SIMD half a page apart, one's
+// matrix instructions beside the other's exponentials, with two barriers a page: 664 us (614 without the offset).
 // Bound: the matrix instructions, with the exponentials beside them.
 template <int D>
 __device__ __forceinline__ int k_at(int row, int ch) { return row * D + ((ch ^ (row & (D / 8 - 1))) << 3); }
