@@ -10,10 +10,12 @@
 //
 // No exponential is taken for a token.  A thread owns 64 neighbouring values; within them they are equally spaced
 // (128 bf16 values share an exponent), so their weights are a geometric series: two exp in 64 bits and 64 products,
-// off by 64 * 2^-53 at most.  All sums are 64-bit and in one fixed order: the same inputs give the same token.
+// off by 64 * 2^-53 at most.  With the counts and weights before each thread's values in LDS, every rule is a search:
+// the thread by two ballots, its 64 values by a scan over a wave's lanes.  All waves make the same searches, so none
+// waits for another.  All sums are 64-bit and in one fixed order: the same inputs give the same token.
 //
-// Bound: HBM for many rows (2 bytes a token), the row's way through one CU for few.  A workgroup of 1024 threads
-// takes a row.
+// Bound: the LDS atomics of the count (about 10 cycles for 64 tokens) and the row's way through one CU, twice.  A
+// workgroup of 1024 threads takes a row, so up to 256 rows take the time of one.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -27,16 +29,18 @@ constexpr int WORDS = BINS / 2;                   // two 16-bit counters a word
 constexpr int CHUNK = 32768;                      // tokens after which counters over 32767 are carried out
 constexpr int CARRIES = 128;                      // carried counts of 32768: rows of up to CARRIES * CHUNK tokens
 
-// 0 for the largest value (all NaN first), 65535 for the smallest; -0 and +0 alike
-__device__ __forceinline__ uint32_t bin_of(uint32_t x) {
-  if (x == 0x8000u) x = 0;
-  return 0xffffu - ((x & 0x8000u) ? (~x & 0xffffu) : (x | 0x8000u));
+// Bins: 0 for the largest value, 65535 for the smallest.  Positive values x (and +NaN first) are bins 0x7fff - x, negative
+// ones stand as they are: +inf is bin 0x7f, +0 0x7fff, -0 0x8000 (its count is moved to +0's), -inf 0xff80.
+constexpr int BIN_INF = 0x7f, BIN_ZERO = 0x7fff, BIN_MINUS_ZERO = 0x8000, BIN_MINUS_INF = 0xff80;
+
+// two tokens at once
+__device__ __forceinline__ uint32_t bins_of(uint32_t x) {
+  const uint32_t neg = (x >> 15) & 0x00010001u;
+  return x ^ (0x7fff7fffu - ((neg << 15) - neg));
 }
 __device__ __forceinline__ float value_of(int bin) {
-  const uint32_t o = 0xffffu - (uint32_t)bin;
-  return __uint_as_float(((o & 0x8000u) ? (o & 0x7fffu) : (~o & 0xffffu)) << 16);
+  return __uint_as_float((uint32_t)(bin < 0x8000 ? 0x7fff - bin : bin) << 16);
 }
-constexpr int BIN_INF = 0xffff - 0xff80;          // of +inf; the bins before it are NaN
 
 // the row in aligned vectors of 8: vector v holds tokens 8v - lead .. 8v - lead + 7, those outside [0, V) are not ours
 struct Row {
@@ -47,48 +51,45 @@ struct Row {
     at = reinterpret_cast<const uint4*>((uintptr_t)p & ~(uintptr_t)15);
     vecs = (V + lead + 7) / 8;
   }
+  // bit e: token e of vector v is ours
+  __device__ uint32_t ours(int v) const {
+    const int lo = max(lead - 8 * v, 0), hi = min(V + lead - 8 * v, 8);
+    return (0xffu >> (8 - hi)) & (0xffu << lo);
+  }
 };
-__device__ __forceinline__ uint32_t half_of(const uint4& v, int e) {
-  const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
-  return (e & 1) ? w >> 16 : w & 0xffffu;
-}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// exclusive sums over the workgroup
 template <class T>
-__device__ __forceinline__ T scan_before(T v, T* red, T* total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  T x = v;
+__device__ __forceinline__ T lane_scan(T v) {      // inclusive, over a wave
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const T y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
+    const T y = __shfl_up(v, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) v += y;
   }
-  if (lane == 63) red[w] = x;
-  __syncthreads();
-  T before = 0, all = 0;
-  for (int i = 0; i < WAVES; ++i) {
-    if (i < w) before += red[i];
-    all += red[i];
-  }
-  __syncthreads();
-  *total = all;
-  // lane 0 starts exactly at the sum of the waves before it
-  const T mine = __shfl_up(x, 1, 64);
-  return before + (lane > 0 ? mine : 0);
+  return v;
 }
 
 struct Shared {
   double red_d[WAVES];
   int red_i[WAVES];
   int first;                   // the largest value's bin
-  int nan;                     // lowest index of a NaN
-  int carries, carry[CARRIES];
-  int rank_p, rank_m, rank, last;
-  double zk, z;
-  int bin, place;              // the answer: a value and which of its tokens
-  double prob;
+  int nan;                     // whether there is a NaN, then its lowest index
+  int carries, carry[CARRIES + 2];
   int in_wave[WAVES];
+  int before_c[NT + 1];        // tokens of the values before each thread's
+  double before_w[NT];         // their weight
 };
+
+// the last thread whose entry is below x (or equal to it, where `equal`); -1 if none.  The entries ascend.
+template <class T>
+__device__ __forceinline__ int last_below(const T* a, T x, bool equal) {
+  const int lane = threadIdx.x & 63;
+  T y = a[lane * (NT / 64)];
+  const int seg = __popcll(__ballot(y < x || (equal && y == x))) - 1;
+  if (seg < 0) return -1;
+  y = a[seg * (NT / 64) + (lane & (NT / 64 - 1))];
+  return seg * (NT / 64) + __popcll(__ballot(y < x || (equal && y == x)) & ((1ull << (NT / 64)) - 1)) - 1;
+}
 
 __global__ void __launch_bounds__(NT)
 sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, const float* __restrict__ uniform,
@@ -98,15 +99,18 @@ sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, const floa
   __shared__ Shared sh;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, b = blockIdx.x;
   const Row row(logits + (size_t)b * ld, V);
+  float T = temperature != nullptr ? temperature[b] : 1.f;
+  int k = top_k != nullptr ? top_k[b] : 0;
+  double p = top_p != nullptr ? (double)top_p[b] : 1.0;
+  double mp = min_p != nullptr ? (double)min_p[b] : 0.0;
+  if (!(T > 0.f)) T = 1.f, k = 1, p = 1.0, mp = 0.0;          // greedy
+  const double u = uniform[b] < 0.f ? 0.0 : (double)uniform[b];
 
   for (int i = t; i < WORDS / 4; i += NT) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
   if (t == 0) {
     sh.first = BINS;
-    sh.nan = INT_MAX;
+    sh.nan = 0;
     sh.carries = 0;
-    sh.rank_p = sh.rank_m = sh.rank = INT_MAX;
-    sh.last = -1;
-    sh.bin = -1;
   }
   __syncthreads();
 
@@ -115,14 +119,14 @@ sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, const floa
     if (v0 > 0) {
       __syncthreads();
       for (int i = t; i < WORDS / 4; i += NT) {
-        uint4 x = reinterpret_cast<uint4*>(hist)[i];
+        const uint4 x = reinterpret_cast<uint4*>(hist)[i];
         if ((x.x | x.y | x.z | x.w) & 0x80008000u) {
           uint32_t* h = &hist[4 * i];
           for (int j = 0; j < 4; ++j)
-            for (int k = 0; k < 2; ++k)
-              if (h[j] & (0x8000u << (16 * k))) {
-                h[j] -= 0x8000u << (16 * k);
-                sh.carry[atomicAdd(&sh.carries, 1)] = 2 * (4 * i + j) + k;
+            for (int c = 0; c < 2; ++c)
+              if (h[j] & (0x8000u << (16 * c))) {
+                h[j] -= 0x8000u << (16 * c);
+                sh.carry[atomicAdd(&sh.carries, 1)] = 2 * (4 * i + j) + c;
               }
         }
       }
@@ -131,222 +135,240 @@ sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, const floa
     const int v1 = min(v0 + CHUNK / 8, row.vecs);
     for (int v = v0 + t; v < v1; v += NT) {
       const uint4 x = row.at[v];
+      const uint32_t ours = row.ours(v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int i = 8 * v + e - row.lead;
-        const uint32_t y = half_of(x, e);
-        if (i < 0 || i >= V || y == 0xff80u) continue;        // -inf: a masked token
-        if ((y & 0x7fffu) > 0x7f80u) {
-          atomicMin(&sh.nan, i);
-          continue;
-        }
-        const uint32_t bin = bin_of(y);
-        atomicAdd(&hist[bin >> 1], 1u << (16 * (bin & 1)));
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t two = bins_of(word_of(x, i)), lo = two & 0xffffu, hi = two >> 16;
+        // masked tokens (-inf) are not counted: they may be most of the row, and on one address
+        if (lo != (uint32_t)BIN_MINUS_INF && (ours == 0xffu || (ours >> (2 * i) & 1))) atomicAdd(&hist[lo >> 1], (lo & 1) ? 0x10000u : 1u);
+        if (hi != (uint32_t)BIN_MINUS_INF && (ours == 0xffu || (ours >> (2 * i + 1) & 1))) atomicAdd(&hist[hi >> 1], (hi & 1) ? 0x10000u : 1u);
       }
     }
   }
   __syncthreads();
-
-  // ---- a thread's 64 values
-  uint32_t cnt2[PER / 2];
-#pragma unroll
-  for (int i = 0; i < PER / 8; ++i) {
-    const uint4 x = reinterpret_cast<const uint4*>(hist)[t * (PER / 8) + i];
-    cnt2[4 * i] = x.x, cnt2[4 * i + 1] = x.y, cnt2[4 * i + 2] = x.z, cnt2[4 * i + 3] = x.w;
+  if (t == 0) {
+    uint32_t c = (hist[BIN_ZERO >> 1] >> 16) + (hist[BIN_MINUS_ZERO >> 1] & 0xffffu);
+    for (int j = 0; j < sh.carries; ++j)
+      if (sh.carry[j] == BIN_MINUS_ZERO) sh.carry[j] = BIN_ZERO;
+    for (; c > 0xffffu; c -= CHUNK) sh.carry[sh.carries++] = BIN_ZERO;
+    hist[BIN_ZERO >> 1] = (hist[BIN_ZERO >> 1] & 0xffffu) | (c << 16);
+    hist[BIN_MINUS_ZERO >> 1] &= 0xffff0000u;
   }
-  auto count = [&](int i) {      // of value t * PER + i
-    int c = (int)((cnt2[i >> 1] >> (16 * (i & 1))) & 0xffffu);
-    return c;
-  };
-  const int ncarry = sh.carries;
-  auto carried = [&](int bin) {  // rare
-    int c = 0;
-    for (int j = 0; j < ncarry; ++j) c += sh.carry[j] == bin ? CHUNK : 0;
-    return c;
-  };
-  auto full = [&](int i) { return count(i) + (ncarry ? carried(t * PER + i) : 0); };
+  __syncthreads();
 
+  // ---- the weight of each thread's 64 values
+  const int ncarry = sh.carries;
+  const int bin0 = t * PER;
+  uint32_t cnt2[PER / 2];
   int mine = BINS;
+  {
+    uint32_t any = 0;
 #pragma unroll
-  for (int i = PER - 1; i >= 0; --i)
-    if (count(i)) mine = t * PER + i;
-  for (int j = 0; j < ncarry; ++j)
-    if (sh.carry[j] / PER == t) mine = min(mine, sh.carry[j]);
-  if (mine < BINS) atomicMin(&sh.first, mine);
+    for (int i = 0; i < PER / 8; ++i) {
+      const uint4 x = reinterpret_cast<const uint4*>(hist)[t * (PER / 8) + i];
+      cnt2[4 * i] = x.x, cnt2[4 * i + 1] = x.y, cnt2[4 * i + 2] = x.z, cnt2[4 * i + 3] = x.w;
+      any |= x.x | x.y | x.z | x.w;
+    }
+    if (any) {
+#pragma unroll
+      for (int i = PER / 2 - 1; i >= 0; --i) {
+        if (cnt2[i] >> 16) mine = bin0 + 2 * i + 1;
+        if (cnt2[i] & 0xffffu) mine = bin0 + 2 * i;
+      }
+    }
+    for (int j = 0; j < ncarry; ++j)
+      if (sh.carry[j] / PER == t) mine = min(mine, sh.carry[j]);
+    // NaN: before +inf, or behind -inf (which is not counted)
+    if (mine < BIN_INF || (mine < BINS && bin0 >= BIN_MINUS_INF)) sh.nan = 1;
+  }
+  int best = mine;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
+  if (lane == 0 && best < BINS) atomicMin(&sh.first, best);
   __syncthreads();
   const int first = sh.first;
-  const int nan = sh.nan;
-  if (nan < V || first == BINS) {      // a NaN counts as the maximum; a row without any token gives -1
+  if (sh.nan || first == BINS) {       // a NaN counts as the maximum; a row without any token gives -1
+    const bool some = sh.nan;
+    __syncthreads();
+    if (t == 0) sh.nan = INT_MAX;
+    __syncthreads();
+    if (some) {
+      for (int v = t; v < row.vecs; v += NT) {
+        const uint4 x = row.at[v];
+        const uint32_t ours = row.ours(v);
+        for (int e = 0; e < 8; ++e)
+          if ((ours >> e & 1) && ((word_of(x, e >> 1) >> (16 * (e & 1))) & 0x7fffu) > 0x7f80u) atomicMin(&sh.nan, 8 * v + e - row.lead);
+      }
+    }
+    __syncthreads();
     if (t == 0) {
-      tokens[b] = nan < V ? nan : -1;
-      probs[b] = nan < V ? NAN : 0.f;
+      tokens[b] = some ? sh.nan : -1;
+      probs[b] = some ? NAN : 0.f;
     }
     return;
   }
   const float vmax = value_of(first);
-  float T = temperature != nullptr ? temperature[b] : 1.f;
-  int k = top_k != nullptr ? top_k[b] : 0;
-  double p = top_p != nullptr ? (double)top_p[b] : 1.0;
-  double mp = min_p != nullptr ? (double)min_p[b] : 0.0;
-  if (!(T > 0.f)) T = 1.f, k = 1, p = 1.0, mp = 0.0;          // greedy
-  const double u = (double)uniform[b];
-
-  // weights of the thread's values from its first one at or below the maximum: w0 * ratio^i
-  const int i0 = min(max(first - t * PER, 0), PER);
-  double w0 = 0.0, ratio = 0.0;
-  if (mine < BINS) {
-    const int bin0 = t * PER + i0;
-    if (bin0 == first) w0 = 1.0;
-    else if (isfinite(vmax)) w0 = exp(((double)value_of(bin0) - (double)vmax) / (double)T);
-    // two neighbours inside the thread's values (a subnormal step is one too); the thread that holds +inf has no
-    // other finite value
-    const int lo = t * PER + PER - 1;
-    if (t * PER > BIN_INF) ratio = exp(((double)value_of(lo) - (double)value_of(lo - 1)) / (double)T);
-  }
+  const double rT = (double)T;
+  // exp((value - max) / T); the largest value's is 1 whatever T and the value are
+  auto weight = [&](int bin) {
+    if (bin == first) return 1.0;
+    return isfinite(vmax) ? exp(((double)value_of(bin) - (double)vmax) / rT) : 0.0;
+  };
   int C = 0;
   double S = 0.0;
-  {
-    double wt = w0;
-    for (int i = i0; i < PER; ++i) {
-      const int c = full(i);
+  if (mine < BINS) {
+    // from the first value at or below the maximum: w0 * ratio^i.  Neighbours are equally spaced (subnormals too); the
+    // thread that holds +inf has no other value to weigh
+    const int i0 = max(first - bin0, 0);
+    const double ratio = bin0 > BIN_INF ? exp(((double)value_of(bin0 + PER - 1) - (double)value_of(bin0 + PER - 2)) / rT) : 0.0;
+    double wt = weight(bin0 + i0);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = (int)((cnt2[i >> 1] >> (16 * (i & 1))) & 0xffffu);
       C += c;
-      S += c * wt;
-      wt *= ratio;
+      S += (double)c * wt;                       // nothing is counted above the maximum
+      if (i >= i0) wt *= ratio;
     }
+    for (int j = 0; j < ncarry; ++j)
+      if (sh.carry[j] / PER == t) {
+        C += CHUNK;
+        S += CHUNK * weight(sh.carry[j]);
+      }
   }
-  int ctotal;
-  double stotal;
-  const int c0 = scan_before(C, sh.red_i, &ctotal);
-  const double s0 = scan_before(S, sh.red_d, &stotal);
-  const int kk = k > 0 ? min(k, ctotal) : ctotal;
+  {
+    const int ci = lane_scan(C);
+    const double si = lane_scan(S);
+    if (lane == 63) sh.red_i[w] = ci, sh.red_d[w] = si;
+    __syncthreads();
+    int c0 = 0;
+    double s0 = 0.0;
+    for (int i = 0; i < w; ++i) {
+      c0 += sh.red_i[i];
+      s0 += sh.red_d[i];
+    }
+    // lane 0 starts exactly at the sum of the waves before it, so that the entries ascend
+    const int cp = __shfl_up(ci, 1, 64);
+    const double sp = __shfl_up(si, 1, 64);
+    sh.before_c[t] = c0 + (lane > 0 ? cp : 0);
+    sh.before_w[t] = s0 + (lane > 0 ? sp : 0.0);
+    if (t == NT - 1) sh.before_c[NT] = c0 + ci;
+    __syncthreads();
+  }
 
-  // weight of the first `n` tokens in order, known to the thread that holds token n - 1
-  auto weight_to = [&](int n, double* to) {
-    if (n > c0 && n <= c0 + C) {
-      int left = n - c0;
-      double x = s0, wt = w0;
-      for (int i = i0; i < PER && left > 0; ++i) {
-        const int c = min(full(i), left);
-        x += c * wt;
-        left -= c;
-        wt *= ratio;
-      }
-      *to = x;
-    }
+  // ---- from here on every wave does the same.  A thread's values in a wave's lanes: count, weight, what is before
+  auto count_of = [&](int bin) {
+    int c = (int)((hist[bin >> 1] >> (16 * (bin & 1))) & 0xffffu);
+    for (int j = 0; j < ncarry; ++j) c += sh.carry[j] == bin ? CHUNK : 0;
+    return c;
   };
-  weight_to(kk, &sh.zk);
-  __syncthreads();
-  const double pz = p * sh.zk;
-  if (C > 0) {
-    // how many tokens have less than p of the mass before them, and how many a weight of at least min_p
-    int np = INT_MAX, nm = INT_MAX, c = c0;
-    double x = s0, wt = w0;
-    for (int i = i0; i < PER; ++i) {
-      const int f = full(i);
-      if (f > 0) {
-        if (p < 1.0 && np == INT_MAX) {
-          if (!(x < pz)) np = c;
-          else if (wt > 0.0) {
-            const double m = ceil((pz - x) / wt);
-            if (m < (double)f) np = c + (int)m;
-          }
-        }
-        if (wt < mp && nm == INT_MAX) nm = c;
-        c += f;
-        x += f * wt;
-      }
-      wt *= ratio;
+  auto all_lanes = [&](double x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+    return x;
+  };
+  // weight of the first n >= 1 tokens in order
+  auto weight_to = [&](int n) {
+    const int thr = last_below(sh.before_c, n, false), bin = thr * PER + lane;
+    const int c = count_of(bin), m = min(max(n - sh.before_c[thr] - (lane_scan(c) - c), 0), c);
+    return sh.before_w[thr] + all_lanes(m > 0 ? m * weight(bin) : 0.0);
+  };
+  const int total = sh.before_c[NT];
+  int keep = k > 0 ? min(k, total) : total;
+  if (p < 1.0) {
+    // tokens that have less than p of the first keep's weight before them
+    const double pz = p * weight_to(keep);
+    const int thr = last_below(sh.before_w, pz, false);
+    int n = 1;
+    if (thr >= 0) {
+      const int bin = thr * PER + lane, c = count_of(bin);
+      const double wt = c > 0 ? weight(bin) : 0.0, cw = c * wt, before = sh.before_w[thr] + (lane_scan(cw) - cw);
+      int m = 0;
+      if (c > 0 && before < pz) m = wt > 0.0 ? (int)min((double)c, ceil((pz - before) / wt)) : c;
+      n = sh.before_c[thr];
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
+      n += m;
     }
-    if (np != INT_MAX) atomicMin(&sh.rank_p, np);
-    if (nm != INT_MAX) atomicMin(&sh.rank_m, nm);
+    keep = max(1, min(keep, n));
   }
-  __syncthreads();
-  const int keep = max(1, min(kk, min(sh.rank_p, sh.rank_m)));
-  weight_to(keep, &sh.z);
-  __syncthreads();
-  const double z = sh.z, target = u * z;
-  int at = -1;                     // the thread's candidate: value, place
-  int place = 0;
-  if (C > 0 && c0 < keep) {
-    int c = c0, last = -1;
-    double x = s0, wt = w0;
-    for (int i = i0; i < PER && c < keep; ++i) {
-      const int f = min(full(i), keep - c);
-      if (f > 0 && wt > 0.0) {
-        if (at < 0 && x + f * wt > target) {
-          at = i;
-          place = min(max((int)floor((target - x) / wt), 0), f - 1);
-          atomicMin(&sh.rank, c + place);
-        }
-        last = c + f - 1;
-      }
-      c += f;
-      x += f * wt;
-      wt *= ratio;
-    }
-    if (last >= 0) atomicMax(&sh.last, last);
+  if (mp > 0.0) {
+    // tokens of a weight of at least min_p: weights fall along the bins, so look at every 1024th, then every 64th of
+    // those, then each
+    auto heavy = [&](int bin) { return bin <= first || weight(bin) >= mp; };
+    const int seg = max(__popcll(__ballot(heavy(lane * (BINS / 64)))) - 1, 0);
+    const int sub = max(__popcll(__ballot(lane < BINS / 64 / PER && heavy(seg * (BINS / 64) + lane * PER))) - 1, 0);
+    const int thr = seg * (BINS / 64 / PER) + sub;
+    int m = heavy(thr * PER + lane) ? count_of(thr * PER + lane) : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
+    keep = max(1, min(keep, sh.before_c[thr] + m));
   }
-  __syncthreads();
-  // u at or past 1, or a NaN: the last kept token that has a weight
-  const int rank = sh.rank != INT_MAX ? sh.rank : sh.last;
-  if (rank >= c0 && rank < c0 + C) {
-    int c = c0;
-    double wt = w0;
-    for (int i = i0; i < PER; ++i) {
-      const int f = full(i);
-      if (rank < c + f) {
-        sh.bin = t * PER + i;
-        sh.place = rank - c;
-        sh.prob = wt / z;
-        break;
-      }
-      c += f;
-      wt *= ratio;
+  const double z = weight_to(keep), target = u * z;
+  int bin = 0, place = 0, in_bin = 0;
+  double prob = 0.0;
+  {
+    // the thread whose weights reach past the target; for u at or past 1 (or a NaN) the last kept token's
+    int thr = target < z ? max(last_below(sh.before_w, target, true), 0) : last_below(sh.before_c, keep, false);
+    for (;; --thr) {       // a thread without a kept token of any weight only at the ends of rounding: the one before
+      const int x = thr * PER + lane, c = count_of(x), ci = lane_scan(c) - c;
+      const int m = min(max(keep - sh.before_c[thr] - ci, 0), c);
+      const double wt = m > 0 ? weight(x) : 0.0, mw = m * wt, before = sh.before_w[thr] + (lane_scan(mw) - mw);
+      const unsigned long long some = __ballot(wt > 0.0), hit = __ballot(wt > 0.0 && before + mw > target);
+      if (some == 0 && thr > 0) continue;
+      const int who = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
+      const int j = hit ? min(max((int)floor((target - before) / wt), 0), m - 1) : m - 1;
+      bin = thr * PER + who;
+      place = __shfl(j, who, 64);
+      in_bin = __shfl(c, who, 64);
+      prob = __shfl(wt, who, 64) / z;
+      break;
     }
   }
-  __syncthreads();
 
   // ---- the token: number `place` among those of the value, by index
-  const uint32_t want = (uint32_t)sh.bin;
-  const int share = (row.vecs + WAVES - 1) / WAVES, v0 = w * share, v1 = min(v0 + share, row.vecs);
+  // a value's tokens are the halves of its bits; of a zero, of its bits without the sign
+  const uint32_t want = bin < 0x8000 ? 0x7fffu - bin : bin, pattern = want | (want << 16);
+  const uint32_t keepbits = bin == BIN_ZERO ? 0x7fff7fffu : 0xffffffffu;
   auto matches = [&](int v) {
     const uint4 x = row.at[v];
     uint32_t mask = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = 8 * v + e - row.lead;
-      const uint32_t y = half_of(x, e);
-      if (i >= 0 && i < V && bin_of(y) == want) mask |= 1u << e;
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t d = (word_of(x, i) & keepbits) ^ pattern;
+      mask |= ((d & 0xffffu) == 0 ? 1u << (2 * i) : 0) | ((d >> 16) == 0 ? 2u << (2 * i) : 0);
     }
-    return mask;
+    return mask & row.ours(v);
   };
+  if (in_bin == 1) {                             // the only one: whoever meets it
+    for (int v = t; v < row.vecs; v += NT) {
+      const uint32_t mask = matches(v);
+      if (mask) {
+        tokens[b] = 8ll * v + (__ffs((int)mask) - 1) - row.lead;
+        probs[b] = (float)prob;
+      }
+    }
+    return;
+  }
+  const int share = (row.vecs + WAVES - 1) / WAVES, v0 = w * share, v1 = min(v0 + share, row.vecs);
   int n = 0;
   for (int v = v0 + lane; v < v1; v += 64) n += __popc(matches(v));
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
   if (lane == 0) sh.in_wave[w] = n;
   __syncthreads();
-  int before = 0;
-  for (int i = 0; i < w; ++i) before += sh.in_wave[i];
-  place = sh.place - before;
+  for (int i = 0; i < w; ++i) place -= sh.in_wave[i];
   if (place < 0 || place >= n) return;           // not this wave
   for (int vb = v0; vb < v1; vb += 64) {
     const int v = vb + lane;
     const uint32_t mask = v < v1 ? matches(v) : 0;
-    int c = __popc(mask), x = c;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(x, o, 64);
-      if (lane >= o) x += y;
-    }
-    const int all = __shfl(x, 63, 64);
+    const int c = __popc(mask), x = lane_scan(c), all = __shfl(x, 63, 64);
     if (place < all) {
       int left = place - (x - c);
       if (left >= 0 && left < c) {
         uint32_t mk = mask;
         while (left-- > 0) mk &= mk - 1;
         tokens[b] = 8ll * v + (__ffs((int)mk) - 1) - row.lead;
-        probs[b] = (float)sh.prob;
+        probs[b] = (float)prob;
       }
       return;
     }
