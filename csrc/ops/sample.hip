@@ -8,14 +8,14 @@
 // logit has at most 2^16 values: a histogram over all of them, held in 128 KB of LDS, is a counting sort of the row.
 // The answer is a rank; the rank is a value and a place among the equal values; a last look at the row finds it.
 //
-// No exponential is taken for a token.  A thread owns 64 neighbouring values; within them they are equally spaced
-// (128 bf16 values share an exponent), so their weights are a geometric series: two exp in 64 bits and 64 products,
-// off by 64 * 2^-53 at most.  With the counts and weights before each thread's values in LDS, every rule is a search:
-// the thread by two ballots, its 64 values by a scan over a wave's lanes.  All waves make the same searches, so none
-// waits for another.  All sums are 64-bit and in one fixed order: the same inputs give the same token.
+// No exponential is taken for a token: only for the values of the 64-value units that hold any, a unit in the lanes of
+// a wave.  With the counts and weights before each unit in LDS, every rule is a search: the unit by two ballots, the
+// value by a scan over the lanes.  All waves make the same searches, so none waits for another.  Weights and sums are
+// 64-bit and in one fixed order: the same inputs give the same token.
 //
-// Bound: the LDS atomics of the count (about 10 cycles for 64 tokens) and the row's way through one CU, twice.  A
-// workgroup of 1024 threads takes a row, so up to 256 rows take the time of one.
+// Bound: the LDS atomics of the count and the row's way into one CU, twice.  A workgroup of 1024 threads takes a row, so
+// up to 256 rows take the time of one.  Measured and left out (152k tokens, 1 row): the row kept in registers, 37 us
+// against 30 -- the loops unrolled for it run from cold instruction lines.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -24,270 +24,351 @@ namespace {
 typedef uint16_t bf16_t;
 
 constexpr int NT = 1024, WAVES = NT / 64;
-constexpr int BINS = 65536, PER = BINS / NT;      // values of a thread
+constexpr int BINS = 65536, UNITS = BINS / 64;
 constexpr int WORDS = BINS / 2;                   // two 16-bit counters a word
-constexpr int CHUNK = 32768;                      // tokens after which counters over 32767 are carried out
-constexpr int CARRIES = 128;                      // carried counts of 32768: rows of up to CARRIES * CHUNK tokens
+constexpr int CARRY = 32768;                      // what is carried out of a counter
+constexpr int CARRIES = 128;                      // carried counts: rows of up to CARRIES * CARRY tokens
+constexpr int BATCH = 4;                          // vectors a thread loads at once: CARRY tokens of a workgroup
+static_assert(BATCH * 8 * NT == CARRY, "a batch of tokens fits a counter of at most 32767 more");
 
-// Bins: 0 for the largest value, 65535 for the smallest.  Positive values x (and +NaN first) are bins 0x7fff - x, negative
-// ones stand as they are: +inf is bin 0x7f, +0 0x7fff, -0 0x8000 (its count is moved to +0's), -inf 0xff80.
-constexpr int BIN_INF = 0x7f, BIN_ZERO = 0x7fff, BIN_MINUS_ZERO = 0x8000, BIN_MINUS_INF = 0xff80;
+// Bins: 0 for the largest value, 65535 for the smallest.  Positive values x (and +NaN first) are bins 0x7fff - x,
+// negative ones (sign bit set) x - 1, so that both zeros are bin 0x7fff.
+constexpr int BIN_INF = 0x7f, BIN_MINUS_INF = 0xff7f;   // behind it: -NaN
+
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+typedef __attribute__((ext_vector_type(2))) int16_t i16x2;
 
 // two tokens at once
 __device__ __forceinline__ uint32_t bins_of(uint32_t x) {
-  const uint32_t neg = (x >> 15) & 0x00010001u;
-  return x ^ (0x7fff7fffu - ((neg << 15) - neg));
+  const uint32_t neg = __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, x) >> (int16_t)15);   // 0xffff or 0
+  const u16x2 y = __builtin_bit_cast(u16x2, x ^ (0x7fff7fffu & ~neg)) + __builtin_bit_cast(u16x2, neg);
+  return __builtin_bit_cast(uint32_t, y);
 }
-__device__ __forceinline__ float value_of(int bin) {
-  return __uint_as_float((uint32_t)(bin < 0x8000 ? 0x7fff - bin : bin) << 16);
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ float value_of(int bin) { return __uint_as_float((uint32_t)(bin < 0x8000 ? 0x7fff - bin : bin + 1) << 16); }
 
-// the row in aligned vectors of 8: vector v holds tokens 8v - lead .. 8v - lead + 7, those outside [0, V) are not ours
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// The row in aligned vectors of 8: vector v holds tokens 8v - lead .. 8v - lead + 7.  A wave has a run of them, 64 a
+// turn, so that the tokens' order is that of the waves, turns, lanes.
 struct Row {
   const uint4* at;
-  int lead, V, vecs;
-  __device__ Row(const bf16_t* p, int V_) : V(V_) {
+  int lead, V, vecs, from;     // from: the wave's first vector
+  __device__ Row(const bf16_t* p, int V_, int turns, int w) : V(V_) {
     lead = (int)(((uintptr_t)p & 15) / 2);
     at = reinterpret_cast<const uint4*>((uintptr_t)p & ~(uintptr_t)15);
     vecs = (V + lead + 7) / 8;
+    from = w * turns * 64;
   }
-  // bit e: token e of vector v is ours
-  __device__ uint32_t ours(int v) const {
-    const int lo = max(lead - 8 * v, 0), hi = min(V + lead - 8 * v, 8);
-    return (0xffu >> (8 - hi)) & (0xffu << lo);
+  // bins that a workgroup sees, those read as masked among them
+  __device__ int seen(int turns) const { return WAVES * turns * 64 * 8; }
+  // all 64 vectors of the turn lie in the row
+  __device__ bool whole(int turn) const { return 8 * (from + 64 * turn) >= lead && 8 * (from + 64 * turn + 64) <= V + lead; }
+  __device__ int vec(int turn) const { return from + 64 * turn + (int)(threadIdx.x & 63); }
+  __device__ __forceinline__ uint4 load(int turn) const { return at[min(vec(turn), vecs - 1)]; }
+  // f(bins of the lane's vector, turn) for all turns, the next batch on its way; before(batch) ahead of each
+  template <class F, class G>
+  __device__ __forceinline__ void each(int turns, F f, G before) const {
+    uint4 x[BATCH], y[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) y[j] = load(j);
+    for (int i = 0; i < turns; i += BATCH) {
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) x[j] = y[j];
+      if (i + BATCH < turns) {
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) y[j] = load(i + BATCH + j);
+      }
+      before(i / BATCH);
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j)
+        if (i + j < turns) f(bins(x[j], i + j), i + j);
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void each(int turns, F f) const { each(turns, f, [](int) {}); }
+  // bins of a turn's vector; what is not the row's reads as masked
+  __device__ __forceinline__ uint4 bins(uint4 x, int turn) const {
+    x = make_uint4(bins_of(x.x), bins_of(x.y), bins_of(x.z), bins_of(x.w));
+    if (!whole(turn)) {
+      auto pair = [&](uint32_t d, int e) {
+        const int i = 8 * vec(turn) + e - lead;
+        if (i < 0 || i >= V) d = (d & 0xffff0000u) | (uint32_t)BIN_MINUS_INF;
+        if (i + 1 < 0 || i + 1 >= V) d = (d & 0xffffu) | ((uint32_t)BIN_MINUS_INF << 16);
+        return d;
+      };
+      x = make_uint4(pair(x.x, 0), pair(x.y, 2), pair(x.z, 4), pair(x.w, 6));
+    }
+    return x;
   }
 };
-__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
+// inclusive sums over a wave's lanes, without LDS: row shifts, then the rows' ends broadcast
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = (uint32_t)moved<CTRL, ROWS>((int)(uint32_t)b), hi = (uint32_t)moved<CTRL, ROWS>((int)(b >> 32));
+  return __builtin_bit_cast(double, (unsigned long long)lo | ((unsigned long long)hi << 32));
+}
 template <class T>
-__device__ __forceinline__ T lane_scan(T v) {      // inclusive, over a wave
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T y = __shfl_up(v, o, 64);
-    if ((int)(threadIdx.x & 63) >= o) v += y;
-  }
+__device__ __forceinline__ T lane_scan(T v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
   return v;
 }
+__device__ __forceinline__ int lane_of(int v, int i) { return __builtin_amdgcn_readlane(v, i); }
+__device__ __forceinline__ double lane_of(double v, int i) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = (uint32_t)lane_of((int)(uint32_t)b, i), hi = (uint32_t)lane_of((int)(b >> 32), i);
+  return __builtin_bit_cast(double, (unsigned long long)lo | ((unsigned long long)hi << 32));
+}
+template <class T>
+__device__ __forceinline__ T lane_sum(T v) { return lane_of(lane_scan(v), 63); }
 
 struct Shared {
   double red_d[WAVES];
   int red_i[WAVES];
-  int first;                   // the largest value's bin
-  int nan;                     // whether there is a NaN, then its lowest index
-  int carries, carry[CARRIES + 2];
-  int in_wave[WAVES];
-  int before_c[NT + 1];        // tokens of the values before each thread's
-  double before_w[NT];         // their weight
+  int first, last;               // the largest and smallest value's bin (greedy rows), the largest one's unit (others)
+  int nan;
+  int counted, masked;           // tokens in the counters, and those that are -inf
+  int index;                     // lowest index of what is looked for
+  int carries, carry[CARRIES];
+  int found[WAVES];
+  int before_c[UNITS + 1];       // a unit's tokens, then the tokens before it
+  double before_w[UNITS + 1];    // their weight
 };
 
-// the last thread whose entry is below x (or equal to it, where `equal`); -1 if none.  The entries ascend.
+// the last unit whose entry is below x (or equal to it, where `equal`); -1 if none.  The entries ascend.
 template <class T>
 __device__ __forceinline__ int last_below(const T* a, T x, bool equal) {
   const int lane = threadIdx.x & 63;
-  T y = a[lane * (NT / 64)];
+  T y = a[lane * (UNITS / 64)];
   const int seg = __popcll(__ballot(y < x || (equal && y == x))) - 1;
   if (seg < 0) return -1;
-  y = a[seg * (NT / 64) + (lane & (NT / 64 - 1))];
-  return seg * (NT / 64) + __popcll(__ballot(y < x || (equal && y == x)) & ((1ull << (NT / 64)) - 1)) - 1;
+  y = a[seg * (UNITS / 64) + (lane & (UNITS / 64 - 1))];
+  return seg * (UNITS / 64) + __popcll(__ballot(y < x || (equal && y == x)) & ((1ull << (UNITS / 64)) - 1)) - 1;
 }
 
 __global__ void __launch_bounds__(NT)
-sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, const float* __restrict__ uniform,
+sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, int turns, const float* __restrict__ uniform,
               const float* __restrict__ temperature, const int* __restrict__ top_k, const float* __restrict__ top_p,
               const float* __restrict__ min_p, int64_t* __restrict__ tokens, float* __restrict__ probs) {
   extern __shared__ __attribute__((aligned(16))) uint32_t hist[];
   __shared__ Shared sh;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, b = blockIdx.x;
-  const Row row(logits + (size_t)b * ld, V);
-  float T = temperature != nullptr ? temperature[b] : 1.f;
-  int k = top_k != nullptr ? top_k[b] : 0;
-  double p = top_p != nullptr ? (double)top_p[b] : 1.0;
-  double mp = min_p != nullptr ? (double)min_p[b] : 0.0;
-  if (!(T > 0.f)) T = 1.f, k = 1, p = 1.0, mp = 0.0;          // greedy
-  const double u = uniform[b] < 0.f ? 0.0 : (double)uniform[b];
-
-  for (int i = t; i < WORDS / 4; i += NT) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), b = blockIdx.x;
+  const Row row(logits + (size_t)b * ld, V, turns, w);
+  const float T = temperature != nullptr ? temperature[b] : 1.f;
   if (t == 0) {
     sh.first = BINS;
-    sh.nan = 0;
-    sh.carries = 0;
+    sh.last = -1;
+    sh.index = INT_MAX;
   }
-  __syncthreads();
 
-  // ---- count
-  for (int v0 = 0; v0 < row.vecs; v0 += CHUNK / 8) {
-    if (v0 > 0) {
-      __syncthreads();
-      for (int i = t; i < WORDS / 4; i += NT) {
-        const uint4 x = reinterpret_cast<uint4*>(hist)[i];
-        if ((x.x | x.y | x.z | x.w) & 0x80008000u) {
-          uint32_t* h = &hist[4 * i];
-          for (int j = 0; j < 4; ++j)
-            for (int c = 0; c < 2; ++c)
-              if (h[j] & (0x8000u << (16 * c))) {
-                h[j] -= 0x8000u << (16 * c);
-                sh.carry[atomicAdd(&sh.carries, 1)] = 2 * (4 * i + j) + c;
-              }
-        }
-      }
-      __syncthreads();
-    }
-    const int v1 = min(v0 + CHUNK / 8, row.vecs);
-    for (int v = v0 + t; v < v1; v += NT) {
-      const uint4 x = row.at[v];
-      const uint32_t ours = row.ours(v);
+  // every token that `wanted` says: the lowest index is the answer; none: -1
+  auto lowest = [&](auto wanted, float prob) {
+    int at = INT_MAX;
+    row.each(turns, [&](const uint4& x, int i) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t two = bins_of(word_of(x, i)), lo = two & 0xffffu, hi = two >> 16;
-        // masked tokens (-inf) are not counted: they may be most of the row, and on one address
-        if (lo != (uint32_t)BIN_MINUS_INF && (ours == 0xffu || (ours >> (2 * i) & 1))) atomicAdd(&hist[lo >> 1], (lo & 1) ? 0x10000u : 1u);
-        if (hi != (uint32_t)BIN_MINUS_INF && (ours == 0xffu || (ours >> (2 * i + 1) & 1))) atomicAdd(&hist[hi >> 1], (hi & 1) ? 0x10000u : 1u);
-      }
-    }
-  }
-  __syncthreads();
-  if (t == 0) {
-    uint32_t c = (hist[BIN_ZERO >> 1] >> 16) + (hist[BIN_MINUS_ZERO >> 1] & 0xffffu);
-    for (int j = 0; j < sh.carries; ++j)
-      if (sh.carry[j] == BIN_MINUS_ZERO) sh.carry[j] = BIN_ZERO;
-    for (; c > 0xffffu; c -= CHUNK) sh.carry[sh.carries++] = BIN_ZERO;
-    hist[BIN_ZERO >> 1] = (hist[BIN_ZERO >> 1] & 0xffffu) | (c << 16);
-    hist[BIN_MINUS_ZERO >> 1] &= 0xffff0000u;
-  }
-  __syncthreads();
-
-  // ---- the weight of each thread's 64 values
-  const int ncarry = sh.carries;
-  const int bin0 = t * PER;
-  uint32_t cnt2[PER / 2];
-  int mine = BINS;
-  {
-    uint32_t any = 0;
-#pragma unroll
-    for (int i = 0; i < PER / 8; ++i) {
-      const uint4 x = reinterpret_cast<const uint4*>(hist)[t * (PER / 8) + i];
-      cnt2[4 * i] = x.x, cnt2[4 * i + 1] = x.y, cnt2[4 * i + 2] = x.z, cnt2[4 * i + 3] = x.w;
-      any |= x.x | x.y | x.z | x.w;
-    }
-    if (any) {
-#pragma unroll
-      for (int i = PER / 2 - 1; i >= 0; --i) {
-        if (cnt2[i] >> 16) mine = bin0 + 2 * i + 1;
-        if (cnt2[i] & 0xffffu) mine = bin0 + 2 * i;
-      }
-    }
-    for (int j = 0; j < ncarry; ++j)
-      if (sh.carry[j] / PER == t) mine = min(mine, sh.carry[j]);
-    // NaN: before +inf, or behind -inf (which is not counted)
-    if (mine < BIN_INF || (mine < BINS && bin0 >= BIN_MINUS_INF)) sh.nan = 1;
-  }
-  int best = mine;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
-  if (lane == 0 && best < BINS) atomicMin(&sh.first, best);
-  __syncthreads();
-  const int first = sh.first;
-  if (sh.nan || first == BINS) {       // a NaN counts as the maximum; a row without any token gives -1
-    const bool some = sh.nan;
-    __syncthreads();
-    if (t == 0) sh.nan = INT_MAX;
-    __syncthreads();
-    if (some) {
-      for (int v = t; v < row.vecs; v += NT) {
-        const uint4 x = row.at[v];
-        const uint32_t ours = row.ours(v);
-        for (int e = 0; e < 8; ++e)
-          if ((ours >> e & 1) && ((word_of(x, e >> 1) >> (16 * (e & 1))) & 0x7fffu) > 0x7f80u) atomicMin(&sh.nan, 8 * v + e - row.lead);
-      }
-    }
+      for (int e = 7; e >= 0; --e)
+        if (wanted((word_of(x, e >> 1) >> (16 * (e & 1))) & 0xffffu)) at = min(at, 8 * row.vec(i) + e - row.lead);
+    });
+    if (at != INT_MAX) atomicMin(&sh.index, at);
     __syncthreads();
     if (t == 0) {
-      tokens[b] = some ? sh.nan : -1;
-      probs[b] = some ? NAN : 0.f;
+      tokens[b] = sh.index != INT_MAX ? sh.index : -1;
+      probs[b] = sh.index != INT_MAX ? prob : 0.f;
     }
+  };
+  // a NaN counts as the maximum
+  auto is_nan = [](uint32_t bin) { return bin < (uint32_t)BIN_INF || bin > (uint32_t)BIN_MINUS_INF; };
+
+  if (!(T > 0.f)) {                // greedy
+    uint32_t lo = 0xffffffffu, hi = 0;
+    row.each(turns, [&](const uint4& x, int) {
+      lo = min2(lo, min2(min2(x.x, x.y), min2(x.z, x.w)));
+      hi = max2(hi, max2(max2(x.x, x.y), max2(x.z, x.w)));
+    });
+    int first = (int)min(lo & 0xffffu, lo >> 16), last = (int)max(hi & 0xffffu, hi >> 16);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      first = min(first, __shfl_xor(first, o, 64));
+      last = max(last, __shfl_xor(last, o, 64));
+    }
+    __syncthreads();
+    if (lane == 0) {
+      atomicMin(&sh.first, first);
+      atomicMax(&sh.last, last);
+    }
+    __syncthreads();
+    first = sh.first;
+    if (first < BIN_INF || sh.last > BIN_MINUS_INF) lowest(is_nan, NAN);
+    else lowest([&](uint32_t bin) { return bin == (uint32_t)first && bin != (uint32_t)BIN_MINUS_INF; }, 1.f);
     return;
   }
-  const float vmax = value_of(first);
+
+  const int k = top_k != nullptr ? top_k[b] : 0;
+  const double p = top_p != nullptr ? (double)top_p[b] : 1.0;
+  const double mp = min_p != nullptr ? (double)min_p[b] : 0.0;
+  const double u = uniform[b] < 0.f ? 0.0 : (double)uniform[b];
   const double rT = (double)T;
+  int first = 0, ncarry = 0;
+  float vmax = 0.f;
   // exp((value - max) / T); the largest value's is 1 whatever T and the value are
   auto weight = [&](int bin) {
     if (bin == first) return 1.0;
     return isfinite(vmax) ? exp(((double)value_of(bin) - (double)vmax) / rT) : 0.0;
   };
-  int C = 0;
-  double S = 0.0;
-  if (mine < BINS) {
-    // from the first value at or below the maximum: w0 * ratio^i.  Neighbours are equally spaced (subnormals too); the
-    // thread that holds +inf has no other value to weigh
-    const int i0 = max(first - bin0, 0);
-    const double ratio = bin0 > BIN_INF ? exp(((double)value_of(bin0 + PER - 1) - (double)value_of(bin0 + PER - 2)) / rT) : 0.0;
-    double wt = weight(bin0 + i0);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int c = (int)((cnt2[i >> 1] >> (16 * (i & 1))) & 0xffffu);
-      C += c;
-      S += (double)c * wt;                       // nothing is counted above the maximum
-      if (i >= i0) wt *= ratio;
-    }
-    for (int j = 0; j < ncarry; ++j)
-      if (sh.carry[j] / PER == t) {
-        C += CHUNK;
-        S += CHUNK * weight(sh.carry[j]);
-      }
-  }
-  {
-    const int ci = lane_scan(C);
-    const double si = lane_scan(S);
-    if (lane == 63) sh.red_i[w] = ci, sh.red_d[w] = si;
-    __syncthreads();
-    int c0 = 0;
-    double s0 = 0.0;
-    for (int i = 0; i < w; ++i) {
-      c0 += sh.red_i[i];
-      s0 += sh.red_d[i];
-    }
-    // lane 0 starts exactly at the sum of the waves before it, so that the entries ascend
-    const int cp = __shfl_up(ci, 1, 64);
-    const double sp = __shfl_up(si, 1, 64);
-    sh.before_c[t] = c0 + (lane > 0 ? cp : 0);
-    sh.before_w[t] = s0 + (lane > 0 ? sp : 0.0);
-    if (t == NT - 1) sh.before_c[NT] = c0 + ci;
-    __syncthreads();
-  }
-
-  // ---- from here on every wave does the same.  A thread's values in a wave's lanes: count, weight, what is before
   auto count_of = [&](int bin) {
     int c = (int)((hist[bin >> 1] >> (16 * (bin & 1))) & 0xffffu);
-    for (int j = 0; j < ncarry; ++j) c += sh.carry[j] == bin ? CHUNK : 0;
+    for (int j = 0; j < ncarry; ++j) c += sh.carry[j] == bin ? CARRY : 0;
     return c;
   };
-  auto all_lanes = [&](double x) {
+
+  // Count, and the units' sums.  A value that more than 65535 tokens have overflows its counter, and then the counts
+  // add up to less than the tokens (a carry into the word's other counter makes up for 1 of 65536): the row is counted
+  // again, this time with full counters carried out as it goes.
+  for (int careful = 0;; ++careful) {
+    for (int i = t; i < WORDS / 4; i += NT) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
+    sh.before_w[t] = 0.0;
+    if (t == 0) {
+      sh.first = BINS;
+      sh.nan = 0;
+      sh.counted = sh.masked = 0;
+      sh.carries = 0;
+    }
+    __syncthreads();
+    auto add = [&](uint32_t bin) { atomicAdd(&hist[bin >> 1], 1u + (bin & 1) * 0xffffu); };
+    int masked = 0;
+    row.each(
+        turns,
+        [&](const uint4& x, int) {
+          const uint32_t top = max2(max2(x.x, x.y), max2(x.z, x.w));
+          const bool some = (top & 0xffffu) >= (uint32_t)BIN_MINUS_INF || (top >> 16) >= (uint32_t)BIN_MINUS_INF;
+          if (!__ballot(some)) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-    return x;
-  };
+            for (int j = 0; j < 4; ++j) {
+              add(word_of(x, j) & 0xffffu);
+              add(word_of(x, j) >> 16);
+            }
+          } else {
+            // masked tokens are not counted: they may be most of the row, and all on one address
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t bin = (word_of(x, j >> 1) >> (16 * (j & 1))) & 0xffffu;
+              if (bin != (uint32_t)BIN_MINUS_INF) add(bin);
+              else ++masked;
+            }
+          }
+        },
+        [&](int batch) {
+          if (!careful || batch == 0) return;
+          __syncthreads();
+          for (int i = t; i < WORDS; i += NT)
+            for (int c = 0; c < 2; ++c)
+              if (hist[i] & (0x8000u << (16 * c))) {
+                hist[i] -= 0x8000u << (16 * c);
+                sh.carry[atomicAdd(&sh.carries, 1)] = 2 * i + c;
+              }
+          __syncthreads();
+        });
+    masked = lane_sum(masked);
+    if (lane == 0 && masked) atomicAdd(&sh.masked, masked);
+    __syncthreads();
+
+    // Unit u is wave u mod WAVES's.  Which hold anything: a lane looks at one, its eight vectors from a place of its own
+    // on, so that the lanes of a read lie on different banks
+    ncarry = __builtin_amdgcn_readfirstlane(sh.carries);
+    const int mine = lane * WAVES + w;
+    int cs = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 x = reinterpret_cast<const uint4*>(hist)[mine * 8 + ((i + lane) & 7)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) cs += (int)((word_of(x, j) & 0xffffu) + (word_of(x, j) >> 16));
+    }
+    for (int j = 0; j < ncarry; ++j) cs += sh.carry[j] / 64 == mine ? CARRY : 0;
+    sh.before_c[mine] = cs;
+    unsigned long long left = __ballot(cs != 0);
+    const int sum = lane_sum(cs);
+    if (left && lane == 0) {
+      atomicMin(&sh.first, __builtin_ctzll(left) * WAVES + w);
+      atomicAdd(&sh.counted, sum);
+    }
+    if (cs != 0 && mine * 64 > BIN_MINUS_INF) sh.nan = 1;
+    __syncthreads();
+    if (!careful && sh.counted != row.seen(turns) - sh.masked) {
+      __syncthreads();
+      continue;
+    }
+    first = sh.first;
+    if (first == BINS) {                         // no token
+      if (t == 0) tokens[b] = -1, probs[b] = 0.f;
+      return;
+    }
+    first = first * 64 + __builtin_ctzll(__ballot(count_of(first * 64 + lane) != 0));
+    if (first < BIN_INF || sh.nan) {
+      lowest(is_nan, NAN);
+      return;
+    }
+    vmax = value_of(first);
+    for (; left != 0; left &= left - 1) {
+      const int unit = __builtin_ctzll(left) * WAVES + w, bin = unit * 64 + lane;
+      const int c = count_of(bin);
+      const double ws = lane_sum(c > 0 ? c * weight(bin) : 0.0);
+      if (lane == 0) sh.before_w[unit] = ws;
+    }
+    __syncthreads();
+    const int c = sh.before_c[t], ci = lane_scan(c);
+    const double s = sh.before_w[t], si = lane_scan(s);
+    if (lane == 63) sh.red_i[w] = ci, sh.red_d[w] = si;
+    __syncthreads();
+    int cb = 0;
+    double sb = 0.0;
+    for (int i = 0; i < w; ++i) {
+      cb += sh.red_i[i];
+      sb += sh.red_d[i];
+    }
+    // an entry is the sum up to the lane before, a wave's first the sum of the waves before, so that they ascend
+    const int cp = __shfl_up(ci, 1, 64);
+    const double sp = __shfl_up(si, 1, 64);
+    sh.before_c[t] = cb + (lane > 0 ? cp : 0);
+    sh.before_w[t] = sb + (lane > 0 ? sp : 0.0);
+    if (t == NT - 1) sh.before_c[UNITS] = cb + ci, sh.before_w[UNITS] = sb + si;
+    __syncthreads();
+    break;
+  }
+
+  // ---- from here on every wave does the same
+  const int total = sh.before_c[UNITS];
   // weight of the first n >= 1 tokens in order
   auto weight_to = [&](int n) {
-    const int thr = last_below(sh.before_c, n, false), bin = thr * PER + lane;
-    const int c = count_of(bin), m = min(max(n - sh.before_c[thr] - (lane_scan(c) - c), 0), c);
-    return sh.before_w[thr] + all_lanes(m > 0 ? m * weight(bin) : 0.0);
+    if (n == total) return sh.before_w[UNITS];
+    const int unit = last_below(sh.before_c, n, false), bin = unit * 64 + lane;
+    const int c = count_of(bin), m = min(max(n - sh.before_c[unit] - (lane_scan(c) - c), 0), c);
+    return sh.before_w[unit] + lane_sum(m > 0 ? m * weight(bin) : 0.0);
   };
-  const int total = sh.before_c[NT];
   int keep = k > 0 ? min(k, total) : total;
   if (p < 1.0) {
     // tokens that have less than p of the first keep's weight before them
     const double pz = p * weight_to(keep);
-    const int thr = last_below(sh.before_w, pz, false);
+    const int unit = last_below(sh.before_w, pz, false);
     int n = 1;
-    if (thr >= 0) {
-      const int bin = thr * PER + lane, c = count_of(bin);
-      const double wt = c > 0 ? weight(bin) : 0.0, cw = c * wt, before = sh.before_w[thr] + (lane_scan(cw) - cw);
+    if (unit >= 0) {
+      const int bin = unit * 64 + lane, c = count_of(bin);
+      const double wt = c > 0 ? weight(bin) : 0.0, cw = c * wt, before = sh.before_w[unit] + (lane_scan(cw) - cw);
       int m = 0;
       if (c > 0 && before < pz) m = wt > 0.0 ? (int)min((double)c, ceil((pz - before) / wt)) : c;
-      n = sh.before_c[thr];
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
-      n += m;
+      n = sh.before_c[unit] + lane_sum(m);
     }
     keep = max(1, min(keep, n));
   }
@@ -296,84 +377,74 @@ sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, const floa
     // those, then each
     auto heavy = [&](int bin) { return bin <= first || weight(bin) >= mp; };
     const int seg = max(__popcll(__ballot(heavy(lane * (BINS / 64)))) - 1, 0);
-    const int sub = max(__popcll(__ballot(lane < BINS / 64 / PER && heavy(seg * (BINS / 64) + lane * PER))) - 1, 0);
-    const int thr = seg * (BINS / 64 / PER) + sub;
-    int m = heavy(thr * PER + lane) ? count_of(thr * PER + lane) : 0;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
-    keep = max(1, min(keep, sh.before_c[thr] + m));
+    const int sub = max(__popcll(__ballot(lane < UNITS / 64 && heavy(seg * (BINS / 64) + lane * 64))) - 1, 0);
+    const int unit = seg * (UNITS / 64) + sub;
+    const int m = lane_sum(heavy(unit * 64 + lane) ? count_of(unit * 64 + lane) : 0);
+    keep = max(1, min(keep, sh.before_c[unit] + m));
   }
   const double z = weight_to(keep), target = u * z;
   int bin = 0, place = 0, in_bin = 0;
   double prob = 0.0;
-  {
-    // the thread whose weights reach past the target; for u at or past 1 (or a NaN) the last kept token's
-    int thr = target < z ? max(last_below(sh.before_w, target, true), 0) : last_below(sh.before_c, keep, false);
-    for (;; --thr) {       // a thread without a kept token of any weight only at the ends of rounding: the one before
-      const int x = thr * PER + lane, c = count_of(x), ci = lane_scan(c) - c;
-      const int m = min(max(keep - sh.before_c[thr] - ci, 0), c);
-      const double wt = m > 0 ? weight(x) : 0.0, mw = m * wt, before = sh.before_w[thr] + (lane_scan(mw) - mw);
-      const unsigned long long some = __ballot(wt > 0.0), hit = __ballot(wt > 0.0 && before + mw > target);
-      if (some == 0 && thr > 0) continue;
-      const int who = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
-      const int j = hit ? min(max((int)floor((target - before) / wt), 0), m - 1) : m - 1;
-      bin = thr * PER + who;
-      place = __shfl(j, who, 64);
-      in_bin = __shfl(c, who, 64);
-      prob = __shfl(wt, who, 64) / z;
-      break;
-    }
+  // the unit whose weights reach past the target; for u at or past 1 (or a NaN) the last kept token's
+  for (int unit = target < z ? last_below(sh.before_w, target, true) : last_below(sh.before_c, keep, false);; --unit) {
+    const int x = unit * 64 + lane, c = count_of(x), ci = lane_scan(c) - c;
+    const int m = min(max(keep - sh.before_c[unit] - ci, 0), c);
+    const double wt = m > 0 ? weight(x) : 0.0, mw = m * wt, before = sh.before_w[unit] + (lane_scan(mw) - mw);
+    const unsigned long long some = __ballot(wt > 0.0), hit = __ballot(wt > 0.0 && before + mw > target);
+    // no kept token of any weight only at the ends of rounding: the unit before.  The first token is kept and weighs 1
+    if (some == 0) continue;
+    const int who = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
+    const int j = hit ? min(max((int)floor((target - before) / wt), 0), m - 1) : m - 1;
+    bin = unit * 64 + who;
+    place = lane_of(j, who);
+    in_bin = lane_of(c, who);
+    prob = lane_of(wt, who) / z;
+    break;
   }
 
   // ---- the token: number `place` among those of the value, by index
-  // a value's tokens are the halves of its bits; of a zero, of its bits without the sign
-  const uint32_t want = bin < 0x8000 ? 0x7fffu - bin : bin, pattern = want | (want << 16);
-  const uint32_t keepbits = bin == BIN_ZERO ? 0x7fff7fffu : 0xffffffffu;
-  auto matches = [&](int v) {
-    const uint4 x = row.at[v];
+  const uint32_t pattern = (uint32_t)bin * 0x10001u;
+  auto answer = [&](int turn, int e) {
+    tokens[b] = 8ll * row.vec(turn) + e - row.lead;
+    probs[b] = (float)prob;
+  };
+  auto matches = [&](const uint4& x) {           // a bit for each token of a vector
     uint32_t mask = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t d = (word_of(x, i) & keepbits) ^ pattern;
+      const uint32_t d = word_of(x, i) ^ pattern;
       mask |= ((d & 0xffffu) == 0 ? 1u << (2 * i) : 0) | ((d >> 16) == 0 ? 2u << (2 * i) : 0);
     }
-    return mask & row.ours(v);
+    return mask;
   };
-  if (in_bin == 1) {                             // the only one: whoever meets it
-    for (int v = t; v < row.vecs; v += NT) {
-      const uint32_t mask = matches(v);
-      if (mask) {
-        tokens[b] = 8ll * v + (__ffs((int)mask) - 1) - row.lead;
-        probs[b] = (float)prob;
-      }
-    }
-    return;
-  }
-  const int share = (row.vecs + WAVES - 1) / WAVES, v0 = w * share, v1 = min(v0 + share, row.vecs);
   int n = 0;
-  for (int v = v0 + lane; v < v1; v += 64) n += __popc(matches(v));
+  row.each(turns, [&](const uint4& x, int i) {
+    uint32_t far = 0x00010001u;                  // 0 in a half where some token matches
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-  if (lane == 0) sh.in_wave[w] = n;
-  __syncthreads();
-  for (int i = 0; i < w; ++i) place -= sh.in_wave[i];
-  if (place < 0 || place >= n) return;           // not this wave
-  for (int vb = v0; vb < v1; vb += 64) {
-    const int v = vb + lane;
-    const uint32_t mask = v < v1 ? matches(v) : 0;
-    const int c = __popc(mask), x = lane_scan(c), all = __shfl(x, 63, 64);
-    if (place < all) {
-      int left = place - (x - c);
-      if (left >= 0 && left < c) {
-        uint32_t mk = mask;
-        while (left-- > 0) mk &= mk - 1;
-        tokens[b] = 8ll * v + (__ffs((int)mk) - 1) - row.lead;
-        probs[b] = (float)prob;
-      }
-      return;
+    for (int j = 0; j < 4; ++j) far = min2(far, word_of(x, j) ^ pattern);
+    if (far != 0x00010001u) {
+      const uint32_t mask = matches(x);
+      if (in_bin == 1) answer(i, __ffs((int)mask) - 1);      // the only one: whoever has it
+      n += (int)__popc(mask);
     }
-    place -= all;
-  }
+  });
+  if (in_bin == 1) return;
+  n = lane_sum(n);
+  if (lane == 0) sh.found[w] = n;
+  __syncthreads();
+  for (int i = 0; i < w; ++i) place -= sh.found[i];
+  if (place < 0 || place >= n) return;           // not this wave
+  row.each(turns, [&](const uint4& x, int i) {
+    const uint32_t mask = matches(x);
+    const int c = (int)__popc(mask), s = lane_scan(c);
+    int left = place - (s - c);
+    if (left >= 0 && left < c) {
+      uint32_t mk = mask;
+      while (left-- > 0) mk &= mk - 1;
+      answer(i, __ffs((int)mk) - 1);
+    }
+    place -= lane_of(s, 63);                     // below 0 behind the answer: no turn matches again
+  });
 }
 
 }  // namespace
@@ -383,12 +454,13 @@ extern "C" {
 int mivgpu_sample(const void* logits, long long ld, int V, int B, const float* uniform, const float* temperature,
                   const int* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* probs,
                   hipStream_t s) {
-  if (B <= 0 || V <= 0 || V > CARRIES * CHUNK || (B > 1 && ld < V)) return -1;
+  if (B <= 0 || V <= 0 || V > CARRIES * CARRY || (B > 1 && ld < V)) return -1;
   constexpr int lds = WORDS * 4;
+  const int turns = ((V + 7 + 7) / 8 + NT - 1) / NT;        // wherever the row starts
   const hipError_t e = hipFuncSetAttribute((const void*)sample_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL(sample_kernel, dim3(B), dim3(NT), lds, s, (const bf16_t*)logits, ld, V, uniform, temperature, top_k,
-                     top_p, min_p, tokens, probs);
+  hipLaunchKernelGGL(sample_kernel, dim3(B), dim3(NT), lds, s, (const bf16_t*)logits, ld, V, turns, uniform, temperature,
+                     top_k, top_p, min_p, tokens, probs);
   return (int)hipGetLastError();
 }
 
