@@ -15,8 +15,11 @@
 // Bound: HBM (the rows once in, q and the codes once out).  Two kinds of workgroups in one launch:
 //   * K/V: one for each kv head and run of up to `window` tokens.  It takes every segment (consecutive slots of one
 //     page) that starts in its run, whole: the page's scale needs all of the segment's values, which 256 threads hold
-//     in registers (64 tokens x D values of K and of V), so nothing is read twice;
-//   * q: one for each token; a thread keeps its 8 sines and cosines for all heads.
+//     in registers (64 tokens x D values of K and of V), so nothing is read twice.  A thread has 8 dimensions of 4 (D =
+//     128) or 2 neighbouring slots, so that its V codes are whole words of V's rows [D][64];
+//   * q: waves of one token each; a lane keeps its 8 sines and cosines for the heads that it walks through.
+// Sines and cosines are the hardware's, which take turns: off by 2^-22.9 at most over [-1/2, 1/2] (all multiples of
+// 2^-22 measured), 40 instructions less than the library's for each of 8 angles.
 #include "paged.h"
 
 using namespace paged;
@@ -38,8 +41,10 @@ __device__ __forceinline__ void angles(int pos, const unsigned long long* __rest
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const unsigned long long f = (unsigned long long)(long long)pos * turns[i0 + e];
-    // the fraction's top 32 bits as a signed half-turn count in [-1, 1): off by 2^-25 of a turn at most
-    sincospif((float)(int)(unsigned)(f >> 32) * 0x1p-31f, &s[e], &c[e]);
+    // the fraction's top 32 bits, signed: turns in [-1/2, 1/2), off by 2^-26 at most as a float
+    const float x = (float)(int)(unsigned)(f >> 32) * 0x1p-32f;
+    s[e] = __builtin_amdgcn_sinf(x);
+    c[e] = __builtin_amdgcn_cosf(x);
   }
 }
 
@@ -69,15 +74,16 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t codes, float f) {
   return to_codes(lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f);
 }
 
-// writes the bytes of `w` whose key (4 * first + i) lies in [lo, hi)
-__device__ __forceinline__ void store_keys(uint8_t* row, int first, uint32_t w, int lo, int hi) {
-  const int k = 4 * first;
-  if (k >= lo && k + 4 <= hi) {
-    *reinterpret_cast<uint32_t*>(row + k) = w;
+// writes the bytes of `w` whose slot (first + i) lies in [lo, hi); BYTES of them, aligned
+template <int BYTES>
+__device__ __forceinline__ void store_slots(uint8_t* row, int first, uint32_t w, int lo, int hi) {
+  if (first >= lo && first + BYTES <= hi) {
+    if (BYTES == 4) *reinterpret_cast<uint32_t*>(row + first) = w;
+    else *reinterpret_cast<uint16_t*>(row + first) = (uint16_t)w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (k + i >= lo && k + i < hi) row[k + i] = (uint8_t)(w >> (8 * i));
+    for (int i = 0; i < BYTES; ++i)
+      if (first + i >= lo && first + i < hi) row[first + i] = (uint8_t)(w >> (8 * i));
   }
 }
 
@@ -87,92 +93,113 @@ append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __rest
               const int* __restrict__ positions, const int* __restrict__ slots,
               const unsigned long long* __restrict__ turns, bf16_t* __restrict__ q_out, uint8_t* __restrict__ kc,
               uint8_t* __restrict__ vc, float* __restrict__ kscale, float* __restrict__ vscale, int N, int Hq, int Hkv,
-              int pages, int window, int nkv, float eps) {
-  constexpr int LANES = Head<D>::LANES, ROWS = Head<D>::ROWS, PASS = PAGE / ROWS;
+              int pages, int window, int nkv, int spread, float eps) {
+  constexpr int LANES = Head<D>::LANES, ROWS = Head<D>::ROWS, PASS = PAGE / ROWS, WROWS = 64 / LANES;
   __shared__ float red[2][NT / 64];
-  __shared__ uint32_t vt[D][PAGE / 4 + 1];       // V codes turned: [dim][key], one word of padding against conflicts
-  const int t = threadIdx.x, l = t % LANES, g = t / LANES;
-  float w[8], c[8], s[8], x[8];
+  const int t = threadIdx.x, lane = t & 63, l = t % LANES;
+  float w[8], c[8], s[8];
 
-  if ((int)blockIdx.x >= nkv) {                  // ---- q heads of one token
-    const int i = blockIdx.x - nkv;
-    angles<D>(positions[i], turns, l, c, s);
+  if ((int)blockIdx.x >= nkv) {                  // ---- q: a wave has every spread-th group of WROWS heads of a token
+    const int x = ((int)blockIdx.x - nkv) * (NT / 64) + (t >> 6), i = x / spread;
+    if (i >= N) return;
+    const bf16_t* row = qkv + (size_t)i * ld + 8 * l;
+    bf16_t* to = q_out + (size_t)i * Hq * D + 8 * l;
     unpack8(*reinterpret_cast<const uint4*>(qw + 8 * l), w);
-    const bf16_t* row = qkv + (size_t)i * ld;
-    for (int h = g; h < (Hq + ROWS - 1) / ROWS * ROWS; h += ROWS) {   // whole waves: the lanes exchange values
-      const bool live = h < Hq;
-      unpack8(*reinterpret_cast<const uint4*>(row + (size_t)min(h, Hq - 1) * D + 8 * l), x);
-      norm_rope<D>(x, w, c, s, l, eps);
-      if (live)
-        *reinterpret_cast<uint4*>(q_out + ((size_t)i * Hq + h) * D + 8 * l) =
-            make_uint4(pack2bf(x[0], x[1]), pack2bf(x[2], x[3]), pack2bf(x[4], x[5]), pack2bf(x[6], x[7]));
+    angles<D>(positions[i], turns, l, c, s);
+    constexpr int AHEAD = 4;                     // heads on their way
+    const int step = WROWS * spread;
+    for (int h0 = x % spread * WROWS + lane / LANES; h0 < Hq + WROWS; h0 += AHEAD * step) {   // whole waves
+      uint4 in[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) in[j] = *reinterpret_cast<const uint4*>(row + (size_t)min(h0 + j * step, Hq - 1) * D);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        float y[8];
+        unpack8(in[j], y);
+        norm_rope<D>(y, w, c, s, l, eps);
+        if (h0 + j * step < Hq)
+          *reinterpret_cast<uint4*>(to + (size_t)(h0 + j * step) * D) =
+              make_uint4(pack2bf(y[0], y[1]), pack2bf(y[2], y[3]), pack2bf(y[4], y[5]), pack2bf(y[6], y[7]));
+      }
     }
     return;
   }
 
   // ---- K/V of one kv head: the segments that start in tokens [i0, i0 + window)
   const int hk = blockIdx.x % Hkv, i0 = (int)(blockIdx.x / Hkv) * window;
-  const int lane = t & 63;
+  const int slot0 = t / LANES * PASS;            // of the thread's PASS slots
   const long long limit = (long long)pages * PAGE;
-  for (int i = i0; i < min(i0 + window, N); ++i) {
-    const int slot = slots[i];
-    if (slot < 0 || slot >= limit) continue;
-    const int off = slot % PAGE;
-    if (off != 0 && i > 0 && slots[i - 1] == slot - 1) continue;      // inside a segment
+  unsigned long long heads;                      // tokens of the run that start a segment
+  {
+    const int i = i0 + lane, slot = lane < window && i < N ? slots[i] : -1;
+    heads = __ballot(slot >= 0 && slot < limit && (slot % PAGE == 0 || i == 0 || slots[max(i - 1, 0)] != slot - 1));
+  }
+  for (; heads != 0; heads &= heads - 1) {
+    const int i = i0 + __ffsll((long long)heads) - 1, slot = slots[i], off = slot % PAGE;
     // its length: tokens whose slots go on in the page
     const bool more = lane + off < PAGE && i + lane < N && slots[min(i + lane, N - 1)] == slot + lane;
     const unsigned long long run = __ballot(more);
-    const int cnt = run == ~0ull ? 64 : __ffsll((long long)~run) - 1;
+    const int cnt = run == ~0ull ? 64 : __ffsll((long long)~run) - 1, end = off + cnt;
     const size_t ph = (size_t)(slot / PAGE) * Hkv + hk;
+    const float ko = off > 0 ? kscale[ph] : 0.f, vo = off > 0 ? vscale[ph] : 0.f;
 
     float kf[PASS][8], vf[PASS][8], ka = 0.f, va = 0.f;
-    unpack8(*reinterpret_cast<const uint4*>(kw + 8 * l), w);
+    const int wslot = (t & ~63) / LANES * PASS;  // the wave's slots: WROWS * PASS from here
+    const bool busy = wslot < end && wslot + WROWS * PASS > off;
+    if (busy) {
+      uint4 kin[PASS], vin[PASS];
+      int pos[PASS];
 #pragma unroll
-    for (int p = 0; p < PASS; ++p) {
-      const int j = p * ROWS + g;
-      const int tok = i + min(j, cnt - 1);
-      const bf16_t* row = qkv + (size_t)tok * ld + ((size_t)Hq + hk) * D + 8 * l;
-      unpack8(*reinterpret_cast<const uint4*>(row), kf[p]);
-      unpack8(*reinterpret_cast<const uint4*>(row + (size_t)Hkv * D), vf[p]);
-      angles<D>(positions[tok], turns, l, c, s);
-      norm_rope<D>(kf[p], w, c, s, l, eps);
-      float kmax = 0.f, vmax = 0.f;
-      bool bad = false;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        kmax = fmaxf(kmax, fabsf(kf[p][e]));
-        vmax = fmaxf(vmax, fabsf(vf[p][e]));
-        bad |= !(fabsf(kf[p][e]) < INFINITY) || !(fabsf(vf[p][e]) < INFINITY);
+      for (int p = 0; p < PASS; ++p) {           // slots outside the segment repeat one of its tokens
+        const int tok = i + min(max(slot0 + p - off, 0), cnt - 1);
+        const bf16_t* row = qkv + (size_t)tok * ld + ((size_t)Hq + hk) * D + 8 * l;
+        kin[p] = *reinterpret_cast<const uint4*>(row);
+        vin[p] = *reinterpret_cast<const uint4*>(row + (size_t)Hkv * D);
+        pos[p] = positions[tok];
       }
-      // any lane of the head row
-      const unsigned long long b = __ballot(bad) >> (lane / LANES * LANES) & ((1ull << LANES) - 1);
-      if (b != 0) {
-        kmax = vmax = 0.f;
+      unpack8(*reinterpret_cast<const uint4*>(kw + 8 * l), w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) kf[p][e] = NAN, vf[p][e] = 0.f;
+      for (int p = 0; p < PASS; ++p) {
+        unpack8(kin[p], kf[p]);
+        unpack8(vin[p], vf[p]);
+        angles<D>(pos[p], turns, l, c, s);
+        norm_rope<D>(kf[p], w, c, s, l, eps);
+        float kmax = 0.f, vmax = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          kmax = fmaxf(kmax, fabsf(kf[p][e]));
+          vmax = fmaxf(vmax, fabsf(vf[p][e]));
+          bad |= !(fabsf(kf[p][e]) < INFINITY) || !(fabsf(vf[p][e]) < INFINITY);
+        }
+        // any lane of the head row
+        const unsigned long long b = __ballot(bad) >> (lane / LANES * LANES) & ((1ull << LANES) - 1);
+        if (b != 0) {
+          kmax = vmax = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) kf[p][e] = NAN, vf[p][e] = 0.f;
+        }
+        ka = fmaxf(ka, kmax);
+        va = fmaxf(va, vmax);
       }
-      ka = fmaxf(ka, kmax);
-      va = fmaxf(va, vmax);
-    }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      ka = fmaxf(ka, __shfl_xor(ka, o, 64));
-      va = fmaxf(va, __shfl_xor(va, o, 64));
+      for (int o = 32; o > 0; o >>= 1) {
+        ka = fmaxf(ka, __shfl_xor(ka, o, 64));
+        va = fmaxf(va, __shfl_xor(va, o, 64));
+      }
     }
     if (lane == 0) red[0][t >> 6] = ka, red[1][t >> 6] = va;
-    __syncthreads();
+    __syncthreads();                             // and every thread has the old scales
     ka = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
     va = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
     float ks = exp2i(scale_exp(ka)), vs = exp2i(scale_exp(va));
     float kr = 1.f, vr = 1.f;                    // what the older codes are multiplied by
     if (off > 0) {
-      const float ko = kscale[ph], vo = vscale[ph];
       if (ko > ks) ks = ko;
       if (vo > vs) vs = vo;
       kr = ko / ks;
       vr = vo / vs;
     }
-    __syncthreads();                             // every thread has the old scales and the maxima
     if (t == 0) kscale[ph] = ks, vscale[ph] = vs;
     const float ki = 1.f / ks, vi = 1.f / vs;    // powers of two: exact
     uint8_t* kp = kc + ph * PAGE * D;
@@ -186,37 +213,30 @@ append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __rest
     if (vr != 1.f) {
       for (int x4 = t; x4 < D * (PAGE / 4); x4 += NT) {
         uint8_t* row = vp + (size_t)(x4 / (PAGE / 4)) * PAGE;
-        const int first = x4 % (PAGE / 4);
-        if (4 * first < off) store_keys(row, first, rescale4(reinterpret_cast<uint32_t*>(row)[first], vr), 0, off);
+        const int first = x4 % (PAGE / 4) * 4;
+        if (first < off) store_slots<4>(row, first, rescale4(*reinterpret_cast<uint32_t*>(row + first), vr), 0, off);
       }
     }
+    if (busy) {
+      const auto fit = [](float y, float inv) { return fminf(fmaxf(y * inv, -448.f), 448.f); };
 #pragma unroll
-    for (int p = 0; p < PASS; ++p) {
-      const int j = p * ROWS + g;
-      if (j < cnt) {
-        const auto fit = [](float y, float inv) { return fminf(fmaxf(y * inv, -448.f), 448.f); };
-        float a[8];
+      for (int p = 0; p < PASS; ++p) {
+        if (slot0 + p < off || slot0 + p >= end) continue;
         const bool nan = kf[p][0] != kf[p][0];   // the whole head row or none of it
+        float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] = fit(kf[p][e], ki);
-        uint2 code = make_uint2(to_codes(a[0], a[1], a[2], a[3]), to_codes(a[4], a[5], a[6], a[7]));
+        for (int e = 0; e < 8; ++e) y[e] = fit(kf[p][e], ki);
+        uint2 code = make_uint2(to_codes(y[0], y[1], y[2], y[3]), to_codes(y[4], y[5], y[6], y[7]));
         if (nan) code = make_uint2(CODE_NAN * 0x01010101u, CODE_NAN * 0x01010101u);
-        *reinterpret_cast<uint2*>(kp + (size_t)(off + j) * D + 8 * l) = code;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] = fit(vf[p][e], vi);
-        const uint32_t lo = to_codes(a[0], a[1], a[2], a[3]), hi = to_codes(a[4], a[5], a[6], a[7]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          reinterpret_cast<uint8_t*>(vt[8 * l + e])[off + j] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
+        *reinterpret_cast<uint2*>(kp + (size_t)(slot0 + p) * D + 8 * l) = code;
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        store_slots<PASS>(vp + (size_t)(8 * l + e) * PAGE, slot0,
+                          to_codes(fit(vf[0][e], vi), fit(vf[1][e], vi), fit(vf[PASS - 2][e], vi), fit(vf[PASS - 1][e], vi)),
+                          off, end);
     }
-    __syncthreads();
-    for (int x4 = t; x4 < D * (PAGE / 4); x4 += NT) {
-      const int dim = x4 / (PAGE / 4), first = x4 % (PAGE / 4);
-      if (4 * first + 4 > off && 4 * first < off + cnt)
-        store_keys(vp + (size_t)dim * PAGE, first, vt[dim][first], off, off + cnt);
-    }
-    __syncthreads();                             // vt and red are free for the next segment
+    __syncthreads();                             // red is free for the next segment
   }
 }
 
@@ -235,12 +255,16 @@ int mivgpu_paged_qk_norm_rope_kv(const void* qkv, long long ld, const void* qw, 
   // segment: runs of 16 keep the workgroups that find nothing few.
   const int window = N <= 1024 ? 1 : 16;
   const long long nkv = (long long)((N + window - 1) / window) * Hkv;
-  if (nkv + N > INT_MAX) return -1;
-  const dim3 grid((unsigned)(nkv + N));
+  // q: few tokens spread their heads over several waves; from 1024 tokens on there are waves enough
+  const int groups = (Hq * head_dim / 8 + 63) / 64;
+  const int spread = N >= 1024 ? 1 : groups < 8 ? groups : 8;
+  const long long nq = ((long long)N * spread + NT / 64 - 1) / (NT / 64);
+  if (nkv + nq > INT_MAX || (long long)N * spread > INT_MAX) return -1;
+  const dim3 grid((unsigned)(nkv + nq));
 #define MIVGPU_APPEND(DD)                                                                                            \
   hipLaunchKernelGGL(append_kernel<DD>, grid, dim3(NT), 0, s, (const bf16_t*)qkv, ld, (const bf16_t*)qw,             \
                      (const bf16_t*)kw, positions, slots, (const unsigned long long*)turns, (bf16_t*)q_out,          \
-                     (uint8_t*)kc, (uint8_t*)vc, kscale, vscale, N, Hq, Hkv, pages, window, (int)nkv, eps)
+                     (uint8_t*)kc, (uint8_t*)vc, kscale, vscale, N, Hq, Hkv, pages, window, (int)nkv, spread, eps)
   if (head_dim == 128) MIVGPU_APPEND(128);
   else if (head_dim == 64) MIVGPU_APPEND(64);
   else return -1;
