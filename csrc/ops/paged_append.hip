@@ -34,15 +34,18 @@ struct Head {
   static constexpr int ROWS = NT / LANES;      // head rows at once
 };
 
-// sines and cosines of the 8 pairs that lane `l` of a head row works on
+// The 8 pairs that lane `l` of a head row works on: their angles as fractions of a turn, times 2^64 ...
 template <int D>
-__device__ __forceinline__ void angles(int pos, const unsigned long long* __restrict__ turns, int l, float* c, float* s) {
-  const int i0 = (l * 8) % (D / 2);
+__device__ __forceinline__ void fractions(int pos, const unsigned long long* __restrict__ turns, int l, unsigned long long* f) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = (unsigned long long)(long long)pos * turns[(l * 8) % (D / 2) + e];
+}
+// ... and their cosines and sines
+__device__ __forceinline__ void angles(const unsigned long long* f, float* c, float* s) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const unsigned long long f = (unsigned long long)(long long)pos * turns[i0 + e];
     // the fraction's top 32 bits, signed: turns in [-1/2, 1/2), off by 2^-26 at most as a float
-    const float x = (float)(int)(unsigned)(f >> 32) * 0x1p-32f;
+    const float x = (float)(int)(unsigned)(f[e] >> 32) * 0x1p-32f;
     s[e] = __builtin_amdgcn_sinf(x);
     c[e] = __builtin_amdgcn_cosf(x);
   }
@@ -88,24 +91,32 @@ __device__ __forceinline__ void store_slots(uint8_t* row, int first, uint32_t w,
 }
 
 template <int D>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, 3)
 append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __restrict__ qw, const bf16_t* __restrict__ kw,
               const int* __restrict__ positions, const int* __restrict__ slots,
               const unsigned long long* __restrict__ turns, bf16_t* __restrict__ q_out, uint8_t* __restrict__ kc,
               uint8_t* __restrict__ vc, float* __restrict__ kscale, float* __restrict__ vscale, int N, int Hq, int Hkv,
-              int pages, int window, int nkv, int spread, float eps) {
+              int pages, int window, unsigned share, int spread, float eps) {
   constexpr int LANES = Head<D>::LANES, ROWS = Head<D>::ROWS, PASS = PAGE / ROWS, WROWS = 64 / LANES;
   __shared__ float red[2][NT / 64];
   const int t = threadIdx.x, lane = t & 63, l = t % LANES;
   float w[8], c[8], s[8];
 
-  if ((int)blockIdx.x >= nkv) {                  // ---- q: a wave has every spread-th group of WROWS heads of a token
-    const int x = ((int)blockIdx.x - nkv) * (NT / 64) + (t >> 6), i = x / spread;
+  // The two kinds take turns, so that the K/V workgroups' latencies lie beside the q workgroups' traffic (8192 tokens: 50
+  // us against 76 with the K/V ones first).  kv: K/V workgroups before this one; share: their part of all, times 2^32
+  const unsigned me = blockIdx.x;
+  const int kv = (int)__umulhi(me, share);
+  if ((int)__umulhi(me + 1, share) == kv) {      // ---- q: a wave has every spread-th group of WROWS heads of a token
+    const int x = ((int)me - kv) * (NT / 64) + (t >> 6), i = x / spread;
     if (i >= N) return;
     const bf16_t* row = qkv + (size_t)i * ld + 8 * l;
     bf16_t* to = q_out + (size_t)i * Hq * D + 8 * l;
     unpack8(*reinterpret_cast<const uint4*>(qw + 8 * l), w);
-    angles<D>(positions[i], turns, l, c, s);
+    {
+      unsigned long long f[8];
+      fractions<D>(positions[i], turns, l, f);
+      angles(f, c, s);
+    }
     constexpr int AHEAD = 4;                     // heads on their way
     const int step = WROWS * spread;
     for (int h0 = x % spread * WROWS + lane / LANES; h0 < Hq + WROWS; h0 += AHEAD * step) {   // whole waves
@@ -126,7 +137,7 @@ append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __rest
   }
 
   // ---- K/V of one kv head: the segments that start in tokens [i0, i0 + window)
-  const int hk = blockIdx.x % Hkv, i0 = (int)(blockIdx.x / Hkv) * window;
+  const int hk = kv % Hkv, i0 = kv / Hkv * window;
   const int slot0 = t / LANES * PASS;            // of the thread's PASS slots
   const long long limit = (long long)pages * PAGE;
   unsigned long long heads;                      // tokens of the run that start a segment
@@ -143,11 +154,13 @@ append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __rest
     const size_t ph = (size_t)(slot / PAGE) * Hkv + hk;
     const float ko = off > 0 ? kscale[ph] : 0.f, vo = off > 0 ? vscale[ph] : 0.f;
 
-    float kf[PASS][8], vf[PASS][8], ka = 0.f, va = 0.f;
+    float kf[PASS][8], ka = 0.f, va = 0.f;
+    uint4 vin[PASS];
+    unsigned bads = 0;                           // of the thread's slots: not finite
     const int wslot = (t & ~63) / LANES * PASS;  // the wave's slots: WROWS * PASS from here
     const bool busy = wslot < end && wslot + WROWS * PASS > off;
     if (busy) {
-      uint4 kin[PASS], vin[PASS];
+      uint4 kin[PASS];
       int pos[PASS];
 #pragma unroll
       for (int p = 0; p < PASS; ++p) {           // slots outside the segment repeat one of its tokens
@@ -158,26 +171,29 @@ append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __rest
         pos[p] = positions[tok];
       }
       unpack8(*reinterpret_cast<const uint4*>(kw + 8 * l), w);
+      unsigned long long f[8];
+      fractions<D>(pos[0], turns, l, f);
 #pragma unroll
       for (int p = 0; p < PASS; ++p) {
         unpack8(kin[p], kf[p]);
-        unpack8(vin[p], vf[p]);
-        angles<D>(pos[p], turns, l, c, s);
+        float vf[8];
+        unpack8(vin[p], vf);
+        if (p > 0) fractions<D>(pos[p], turns, l, f);
+        angles(f, c, s);
         norm_rope<D>(kf[p], w, c, s, l, eps);
         float kmax = 0.f, vmax = 0.f;
         bool bad = false;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           kmax = fmaxf(kmax, fabsf(kf[p][e]));
-          vmax = fmaxf(vmax, fabsf(vf[p][e]));
-          bad |= !(fabsf(kf[p][e]) < INFINITY) || !(fabsf(vf[p][e]) < INFINITY);
+          vmax = fmaxf(vmax, fabsf(vf[e]));
+          bad |= !(fabsf(kf[p][e]) < INFINITY) || !(fabsf(vf[e]) < INFINITY);
         }
         // any lane of the head row
         const unsigned long long b = __ballot(bad) >> (lane / LANES * LANES) & ((1ull << LANES) - 1);
         if (b != 0) {
           kmax = vmax = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) kf[p][e] = NAN, vf[p][e] = 0.f;
+          bads |= 1u << p;
         }
         ka = fmaxf(ka, kmax);
         va = fmaxf(va, vmax);
@@ -222,19 +238,24 @@ append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __rest
 #pragma unroll
       for (int p = 0; p < PASS; ++p) {
         if (slot0 + p < off || slot0 + p >= end) continue;
-        const bool nan = kf[p][0] != kf[p][0];   // the whole head row or none of it
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = fit(kf[p][e], ki);
         uint2 code = make_uint2(to_codes(y[0], y[1], y[2], y[3]), to_codes(y[4], y[5], y[6], y[7]));
-        if (nan) code = make_uint2(CODE_NAN * 0x01010101u, CODE_NAN * 0x01010101u);
+        if (bads >> p & 1) code = make_uint2(CODE_NAN * 0x01010101u, CODE_NAN * 0x01010101u);
         *reinterpret_cast<uint2*>(kp + (size_t)(slot0 + p) * D + 8 * l) = code;
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        store_slots<PASS>(vp + (size_t)(8 * l + e) * PAGE, slot0,
-                          to_codes(fit(vf[0][e], vi), fit(vf[1][e], vi), fit(vf[PASS - 2][e], vi), fit(vf[PASS - 1][e], vi)),
-                          off, end);
+      for (int p = 0; p < PASS; ++p)
+        if (bads >> p & 1) vin[p] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        auto code = [&](int p) {
+          const uint32_t x = e < 2 ? vin[p].x : e < 4 ? vin[p].y : e < 6 ? vin[p].z : vin[p].w;
+          return fit(__uint_as_float((e & 1) ? x & 0xffff0000u : x << 16), vi);
+        };
+        store_slots<PASS>(vp + (size_t)(8 * l + e) * PAGE, slot0, to_codes(code(0), code(1), code(PASS - 2), code(PASS - 1)), off, end);
+      }
     }
     __syncthreads();                             // red is free for the next segment
   }
@@ -251,9 +272,9 @@ int mivgpu_paged_qk_norm_rope_kv(const void* qkv, long long ld, const void* qw, 
   if (N < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || pages <= 0 || (long long)pages * PAGE > INT_MAX) return -1;
   if (ld < (long long)(Hq + 2 * Hkv) * head_dim || ld % 8) return -1;
   if (N == 0) return 0;
-  // A decode step has a segment for each token: a workgroup for each.  In a long batch most tokens lie inside a
-  // segment: runs of 16 keep the workgroups that find nothing few.
-  const int window = N <= 1024 ? 1 : 16;
+  // A decode step has a segment for each token: a workgroup for each.  In a longer batch (of at most 1024 requests, as
+  // everywhere here) ever more tokens lie inside segments: runs of 16 or 64 keep the workgroups that find nothing few.
+  const int window = N <= 1024 ? 1 : N < 4096 ? 16 : 64;
   const long long nkv = (long long)((N + window - 1) / window) * Hkv;
   // q: few tokens spread their heads over several waves; from 1024 tokens on there are waves enough
   const int groups = (Hq * head_dim / 8 + 63) / 64;
@@ -261,10 +282,12 @@ int mivgpu_paged_qk_norm_rope_kv(const void* qkv, long long ld, const void* qw, 
   const long long nq = ((long long)N * spread + NT / 64 - 1) / (NT / 64);
   if (nkv + nq > INT_MAX || (long long)N * spread > INT_MAX) return -1;
   const dim3 grid((unsigned)(nkv + nq));
+  // rounded up: share * all >> 32 is nkv, and one more K/V workgroup at most from one workgroup to the next (nq > 0)
+  const unsigned share = (unsigned)((((unsigned long long)nkv << 32) + (nkv + nq) - 1) / (nkv + nq));
 #define MIVGPU_APPEND(DD)                                                                                            \
   hipLaunchKernelGGL(append_kernel<DD>, grid, dim3(NT), 0, s, (const bf16_t*)qkv, ld, (const bf16_t*)qw,             \
                      (const bf16_t*)kw, positions, slots, (const unsigned long long*)turns, (bf16_t*)q_out,          \
-                     (uint8_t*)kc, (uint8_t*)vc, kscale, vscale, N, Hq, Hkv, pages, window, (int)nkv, spread, eps)
+                     (uint8_t*)kc, (uint8_t*)vc, kscale, vscale, N, Hq, Hkv, pages, window, share, spread, eps)
   if (head_dim == 128) MIVGPU_APPEND(128);
   else if (head_dim == 64) MIVGPU_APPEND(64);
   else return -1;
