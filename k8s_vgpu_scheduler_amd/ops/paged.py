@@ -104,14 +104,21 @@ def page_plan(new_lens: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
     pages = free.numel()
     if n_tokens < 0 or max(pages, W) * PAGE > 2**31 - 1:
         raise ValueError(f"page_plan: n_tokens {n_tokens}, {pages} pages, {W} a request: slots are 32-bit")
-    if out is None:
-        buf = torch.empty(3 * B + 1 + 2 * n_tokens, dtype=_I32, device=table.device)     # one allocation
-        out = PagePlan(*torch.split_with_sizes(buf, (B + 1, B, B, n_tokens, n_tokens)))
     idx, p = _ptrs("page_plan", ("new_lens", new_lens, _I32, (B,)), ("lengths", lengths, _I32, (B,)),
-                   ("table", table, _I32, (B, W)), ("free", free, _I32, (pages,)), ("ring", ring, _I32, (2,)),
-                   ("cu_q", out.cu_q, _I32, (B + 1,)), ("kv_lens", out.kv_lens, _I32, (B,)),
-                   ("taken", out.taken, _I32, (B,)), ("positions", out.positions, _I32, (n_tokens,)),
-                   ("slots", out.slots, _I32, (n_tokens,)))
+                   ("table", table, _I32, (B, W)), ("free", free, _I32, (pages,)), ("ring", ring, _I32, (2,)))
+    sizes = (B + 1, B, B, n_tokens, n_tokens)
+    if out is None:
+        buf = torch.empty(sum(sizes), dtype=_I32, device=table.device)     # one allocation
+        out = PagePlan(*torch.split_with_sizes(buf, sizes))
+        at = buf.data_ptr()
+        for n in sizes:
+            p.append(at)
+            at += 4 * n
+    else:
+        on, more = _ptrs("page_plan", *((what, t, _I32, (n,)) for what, t, n in zip(PagePlan._fields, out, sizes)))
+        if on != idx:
+            raise ValueError("page_plan: every tensor must be on one GPU")
+        p += more
     _launch(idx, "page_plan", ops.lib().mivgpu_page_plan, *p, B, W, pages, n_tokens)
     return out
 
