@@ -13,7 +13,7 @@
 // (m, l, O) in the workspace, and the last one to arrive (a counter that it sets back to zero) joins them in the order
 // of the parts, so that a call's bits do not depend on who that is.
 //
-// Tiles of 16: the four waves of a workgroup take every fourth page and join in LDS.  Per page of 64 keys a wave
+// Tiles of 16: the eight waves of a workgroup take every eighth page and join in LDS.  Per page of 64 keys a wave
 // computes, with 16x16x32 bf16 MFMAs,
 //   S^T (64 keys x 16 rows) = K . Q^T        4 tiles of 16 keys: tile t's row 4a + c is key 16a + 4t + c, so that
 //                                            lane (row r, quarter a) ends with the 16 consecutive keys 16a .. 16a+15;
@@ -34,16 +34,17 @@ typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 
 // short requests
-constexpr int NT = 256, WAVES = 4, TILE = 16;
+constexpr int WAVES = 8, NT = 64 * WAVES, TILE = 16;
 constexpr int MIN_CHUNK = WAVES;         // pages of a part: at least one for each wave
 constexpr int MAX_PARTS = 256;           // of a tile: their (m, l) take 32 KB of LDS
+constexpr int JOIN = 64;                 // head dimensions that the waves join at once
 constexpr int SHORT_ROWS = 64;
 // long requests
 constexpr int LNT = 512, LWAVES = 8, LTILE = 32 * LWAVES;
 constexpr int LMIN_CHUNK = 8;
 
-// Workgroups that a call aims at (two a CU, one a CU), over all kv heads, and with them the slots of the workspace.
-// With t parts aimed at a kv head a split tile of np pages gets at most np / chunk + 1 <= 2 np / chunk parts, which
+// A call aims at as many workgroups as are resident (two of the short ones with D = 64 a CU, otherwise one), over all kv
+// heads, and with that bounds the slots of the workspace: with t parts aimed at a kv head a split tile of np pages gets at most np / chunk + 1 <= 2 np / chunk parts, which
 // add up to at most 2 t.
 constexpr int MAX_CUS = 256, MAX_HKV = 256;
 constexpr int SHORT_SLOTS = 2 * 2 * MAX_CUS, LONG_SLOTS = 2 * MAX_CUS;
@@ -161,7 +162,7 @@ __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const in
 }
 
 template <int D>
-__global__ void __launch_bounds__(NT, 2)
+__global__ void __launch_bounds__(NT, D == 64 ? 4 : 2)
 attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
             const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ table,
             const int* __restrict__ cu, const int* __restrict__ kv_lens, bf16_t* __restrict__ out,
@@ -171,14 +172,14 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
   constexpr int DT = D / 16;              // output tiles
   __shared__ float s_m[WAVES][TILE], s_l[WAVES][TILE];
   // the waves' O; later the (m, l) of a tile's parts and what groups of threads make of them
-  constexpr int O_BYTES = WAVES * TILE * (D + 4) * 4, JOIN_BYTES = MAX_PARTS * TILE * 8 + NT * 20;
+  constexpr int O_BYTES = WAVES * TILE * (JOIN + 4) * 4, JOIN_BYTES = MAX_PARTS * TILE * 8 + NT * 20;
   __shared__ __attribute__((aligned(16))) char s_raw[O_BYTES > JOIN_BYTES ? O_BYTES : JOIN_BYTES];
-  float(*s_o)[TILE][D + 4] = reinterpret_cast<float(*)[TILE][D + 4]>(s_raw);
+  float(*s_o)[TILE][JOIN + 4] = reinterpret_cast<float(*)[TILE][JOIN + 4]>(s_raw);
   __shared__ int s_last;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 15, a = lane >> 4;
-  const int G = Hq / Hkv, hk = blockIdx.y;
-  const Share sh = find_share<TILE, MIN_CHUNK>(cu, kv_lens, N, B, W, G, target, 0, upto, blockIdx.x);
+  const int G = Hq / Hkv, hk = blockIdx.x % Hkv;
+  const Share sh = find_share<TILE, MIN_CHUNK>(cu, kv_lens, N, B, W, G, target, 0, upto, blockIdx.x / Hkv);
   if (sh.ns == 0) return;
   const int b = sh.b, row0 = sh.tile * TILE, ns = sh.ns;
   const int tok0 = min(max(cu[b], 0), N), n = min(cu[b + 1], N) - tok0, rows = n * G;
@@ -322,32 +323,37 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
   if (a == 0) s_m[w][r] = m, s_l[w][r] = l;
-#pragma unroll
-  for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4_t*>(&s_o[w][r][16 * i + 4 * a]) = o[i];
-  __syncthreads();
   const size_t slot0 = (size_t)sh.slot * Hkv + hk, slot_step = Hkv;     // the tile's parts in the workspace
   const size_t slot = slot0 + sh.part * slot_step;
-  for (int x = t; x < TILE * (D / 4); x += NT) {
-    const int rr = x / (D / 4), d = x % (D / 4) * 4;
-    if (row0 + rr >= rows) continue;
-    float mm = -INFINITY;
+  const int filled = min(TILE, rows - row0);
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) mm = fmaxf(mm, s_m[i][rr]);
-    const float base = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f;
-    f32x4_t oo = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < D / JOIN; ++j) {
+    if (j > 0) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) {
-      const float f = __builtin_amdgcn_exp2f(s_m[i][rr] - base);
-      ll += s_l[i][rr] * f;
-      oo += *reinterpret_cast<const f32x4_t*>(&s_o[i][rr][d]) * f;
-    }
-    if (ns == 1) {
-      store_row(out, oo, ll, row0 + rr, tok0, G, Hq, hk, D, d);
-    } else {
-      put2(part_o + (slot * TILE + rr) * D + d, oo[0], oo[1]);
-      put2(part_o + (slot * TILE + rr) * D + d + 2, oo[2], oo[3]);
-      if (d == 0) put2(part_ml + (slot * TILE + rr) * 2, mm, ll);
+    for (int i = 0; i < JOIN / 16; ++i)
+      if (r < filled) *reinterpret_cast<f32x4_t*>(&s_o[w][r][16 * i + 4 * a]) = o[JOIN / 16 * j + i];
+    __syncthreads();
+    const int rr = t / (JOIN / 4), d = t % (JOIN / 4) * 4;             // a thread's row and four dimensions
+    if (rr < filled) {
+      float mm = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) mm = fmaxf(mm, s_m[i][rr]);
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f;
+      f32x4_t oo = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) {
+        const float f = __builtin_amdgcn_exp2f(s_m[i][rr] - base);
+        ll += s_l[i][rr] * f;
+        oo += *reinterpret_cast<const f32x4_t*>(&s_o[i][rr][d]) * f;
+      }
+      if (ns == 1) {
+        store_row(out, oo, ll, row0 + rr, tok0, G, Hq, hk, D, JOIN * j + d);
+      } else {
+        put2(part_o + (slot * TILE + rr) * D + JOIN * j + d, oo[0], oo[1]);
+        put2(part_o + (slot * TILE + rr) * D + JOIN * j + d + 2, oo[2], oo[3]);
+        if (j == 0 && d == 0) put2(part_ml + (slot * TILE + rr) * 2, mm, ll);
+      }
     }
   }
   if (ns == 1) return;
@@ -362,32 +368,37 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
   if (!s_last) return;
   if (t == 0) __hip_atomic_store(&counters[slot0], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   const int live = min(TILE, rows - row0);
+  // Four values a thread; few rows leave threads over, and each of `groups` takes every groups-th part.  The first parts'
+  // O are on their way while all (m, l) come into LDS.
   float2* ml = reinterpret_cast<float2*>(s_raw);                      // [part][row]
   float* joined = reinterpret_cast<float*>(s_raw + MAX_PARTS * TILE * 8);   // [thread][4 values, l]
-  for (int x = t; x < ns * live; x += NT) {
-    const int i = x / live, rr = x % live;
-    ml[i * TILE + rr] = get2(part_ml + ((slot0 + i * slot_step) * TILE + rr) * 2);
+  const int units = filled * (D / 4), groups = max(NT / units, 1);
+  static_assert(TILE * D / 4 <= NT, "a thread for every four values");
+  const int group = t / units, unit = t - group * units, rr = unit / (D / 4), d = unit % (D / 4) * 4;
+  constexpr int AHEAD = 8;                        // loads in flight
+  float2 x01[AHEAD], x23[AHEAD];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const float* src = part_o + ((slot0 + min(i0 + j * groups, ns - 1) * slot_step) * TILE + rr) * D + d;
+      x01[j] = get2(src);
+      x23[j] = get2(src + 2);
+    }
+  };
+  if (group < groups) load(group);
+  for (int x = t; x < ns * filled; x += NT) {
+    const int i = x / filled, row = x % filled;
+    ml[i * TILE + row] = get2(part_ml + ((slot0 + i * slot_step) * TILE + row) * 2);
   }
   __syncthreads();
-  // four values a thread; few rows leave threads over, and each of `groups` takes every groups-th part
-  const int units = live * (D / 4), groups = max(NT / units, 1);
-  for (int x = t; x < units * groups; x += NT) {
-    const int unit = x % units, group = x / units, rr = unit / (D / 4), d = unit % (D / 4) * 4;
+  if (group < groups) {
     float mm = -INFINITY;
     for (int i = 0; i < ns; ++i) mm = fmaxf(mm, ml[i * TILE + rr].x);
     const float base = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f;
     f32x4_t oo = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const float* at = part_o + (slot0 * TILE + rr) * D + d;
-    constexpr int AHEAD = 8;                      // loads in flight
     for (int i0 = group; i0 < ns; i0 += groups * AHEAD) {
-      float2 x01[AHEAD], x23[AHEAD];
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        const float* src = at + (size_t)min(i0 + j * groups, ns - 1) * slot_step * TILE * D;
-        x01[j] = get2(src);
-        x23[j] = get2(src + 2);
-      }
+      if (i0 != group) load(i0);
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         const int i = i0 + j * groups;
@@ -401,10 +412,10 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
     }
     if (groups == 1) {
       store_row(out, oo, ll, row0 + rr, tok0, G, Hq, hk, D, d);
-    } else {                                      // units * groups <= NT: one turn
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) joined[x * 5 + j] = oo[j];
-      joined[x * 5 + 4] = ll;
+      for (int j = 0; j < 4; ++j) joined[t * 5 + j] = oo[j];
+      joined[t * 5 + 4] = ll;
     }
   }
   if (groups == 1) return;
@@ -709,11 +720,13 @@ int mivgpu_paged_attention(const void* q, const void* kc, const void* vc, const 
     const long long all = tiles * ((W + chunk - 1) / chunk), most = tiles + target;
     return all < most ? all : most;
   };
-  const int target = 2 * all_cus() / Hkv > 1 ? 2 * all_cus() / Hkv : 1, ltarget = all_cus() / Hkv > 1 ? all_cus() / Hkv : 1;
-  long long tiles = rows / TILE + some;
+  const int ltarget = all_cus() / Hkv > 1 ? all_cus() / Hkv : 1;
+  const int resident = head_dim == 64 ? 2 * all_cus() : all_cus(), target = resident / Hkv > 1 ? resident / Hkv : 1;
+  long long tiles = rows / TILE + some, each = (long long)N * ((G + TILE - 1) / TILE);
+  if (tiles > each) tiles = each;          // a token adds no more tiles than its own rows fill
   if (longs && tiles > some * (SHORT_ROWS / TILE)) tiles = some * (SHORT_ROWS / TILE);
   const long long few = rows / (SHORT_ROWS + 1), ltiles = rows / LTILE + (few < some ? few : some);
-  const long long parts = grid_of(tiles, target, MIN_CHUNK), lparts = grid_of(ltiles, ltarget, LMIN_CHUNK) * Hkv;
+  const long long parts = grid_of(tiles, target, MIN_CHUNK) * Hkv, lparts = grid_of(ltiles, ltarget, LMIN_CHUNK) * Hkv;
   if (tiles * W > INT_MAX || (longs && ltiles * W > INT_MAX) || parts > INT_MAX || lparts > INT_MAX) return -1;
 #define MIVGPU_PATTN(DD)                                                                                              \
   do {                                                                                                                \
@@ -721,7 +734,7 @@ int mivgpu_paged_attention(const void* q, const void* kc, const void* vc, const 
       hipLaunchKernelGGL(attn_long_kernel<DD>, dim3((unsigned)lparts), dim3(LNT), 0, s, (const bf16_t*)q,             \
                          (const uint8_t*)kc, (const uint8_t*)vc, kscale, vscale, table, cu, kv_lens, (bf16_t*)out,    \
                          (int*)work + SHORT_SLOTS, lml, lo, N, B, W, Hq, Hkv, pages, ltarget, sl2);                   \
-    hipLaunchKernelGGL(attn_kernel<DD>, dim3((unsigned)parts, Hkv), dim3(NT), 0, s, (const bf16_t*)q,                 \
+    hipLaunchKernelGGL(attn_kernel<DD>, dim3((unsigned)parts), dim3(NT), 0, s, (const bf16_t*)q,                      \
                        (const uint8_t*)kc, (const uint8_t*)vc, kscale, vscale, table, cu, kv_lens, (bf16_t*)out,      \
                        (int*)work, sml, so, N, B, W, Hq, Hkv, pages, target, longs ? SHORT_ROWS : INT_MAX, sl2);      \
   } while (0)
