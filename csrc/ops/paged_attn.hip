@@ -117,13 +117,16 @@ __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const in
       }
     }
   };
-  int sum = 0;
+  int sum = 0, some = 0;
   for (int i = 0; i < per; ++i) {
     size(lane * per + i);
     sum += tiles * np;
+    some += tiles;
   }
   const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
-  const int chunk = max((total + target - 1) / target, SMALLEST);
+  // a tile's last part is mostly smaller than a chunk: leave a workgroup for each, so that all parts are resident at once
+  const int goal = max(target - __builtin_amdgcn_readlane(wave_scan(some), 63), (target + 1) / 2);
+  const int chunk = max((total + goal - 1) / goal, SMALLEST);
   auto parts = [&](int pages) { return min(max((pages + chunk - 1) / chunk, 1), MAX_PARTS); };
   int split = 0;
   sum = 0;
