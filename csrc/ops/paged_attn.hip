@@ -22,6 +22,7 @@
 // (exact: a code has 4 significant bits and the scale is a power of two).  P is rounded to bf16 (half a step of the
 // output's type, before a sum that averages it); scores, m, l and O stay in fp32.
 #include "paged.h"
+#include <type_traits>
 
 using namespace paged;
 
@@ -60,6 +61,15 @@ __device__ __forceinline__ bf16x8_t widen(uint32_t lo, uint32_t hi, float s) {
 __device__ __forceinline__ uint32_t live_bytes(int k0, int live) {
   const int n = min(max(live - k0, 0), 4);
   return n == 4 ? ~0u : (1u << (8 * n)) - 1u;
+}
+
+// waits for a loaded operand here.  Without it the compiler waits wherever a loop uses the operand, there for the loads
+// that the loop itself has on their way
+__device__ __forceinline__ void arrived(bf16x8_t& x) {
+  typedef __attribute__((ext_vector_type(4))) int i32x4_t;
+  i32x4_t y = __builtin_bit_cast(i32x4_t, x);
+  asm volatile("" : "+v"(y));
+  x = __builtin_bit_cast(bf16x8_t, y);
 }
 
 // two floats to and from memory that workgroups on other XCDs share within a launch
@@ -437,20 +447,25 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
 
 // ------------------------------------------------------------------------------------------------ long requests --
 // Eight waves of 32 rows share every page: its codes become bf16 once, on their way from registers (a 16-byte load
-// of K and of V a thread, a page ahead) to LDS, double-buffered with one barrier a page.  Per page a wave computes,
-// with 32x32x16 bf16 MFMAs,
+// of K and of V a thread) to LDS.  LDS has room for four pages: between the two pages that are worked on, the next two
+// are stored and the loads of the two after those sent off; one barrier for two pages.  Per page a wave computes, with
+// 32x32x16 bf16 MFMAs,
 //   S^T (2 x 32 keys x 32 rows) = K . Q^T     lane (row r, half h) holds the keys (i & 3) + 8 (i >> 2) + 4 h of each 32;
 //   O^T (D x 32 rows) += V^T . P^T            eight registers of S^T are the operand of a k-step of 16 keys: keys
 //                                             {0-3, 8-11} + 4 h; V's 16 keys are stored in two chunks in that order.
-// LDS rows are permuted by 16-byte chunks (chunk ^ row) so that the lanes of a read cover all banks.
+// LDS rows are permuted by 16-byte chunks (chunk ^ row; V's, two rows to the banks, chunk ^ row / 2) so that the lanes
+// of a read cover all banks.
 // The output and sum are rescaled only where a row's maximum grew by more than 8 (in log2): the p stay below 2^8,
 // which neither bf16 nor the sums mind.
-// Measured and left out (8192-token prompt, this kernel 565 us): the two waves of a SIMD half a page apart, one's
-// matrix instructions beside the other's exponentials, with two barriers a page: 664 us (614 without the offset).
-// Bound: the matrix instructions, with the exponentials beside them.
+// Measured on an 8192-token prompt, 32 / 8 heads: 515 us, 1067 TFLOP/s; with the stores before the barrier instead of
+// between the pages 525, a barrier a page 568, the buffers picked at run time 551.  The matrix units are busy less than
+// half of the time, the softmax of a SIMD's two waves and the stores take the rest: without the stores and loads it
+// would be 396.  Left out: the two waves of a SIMD half a page apart, one's matrix instructions beside the other's
+// exponentials, two barriers a page (653; 614 without the offset); four waves of 64 rows, which halve the LDS reads,
+// the next page's scores beside this one's exponentials (792).
 template <int D>
 __device__ __forceinline__ int k_at(int row, int ch) { return row * D + ((ch ^ (row & (D / 8 - 1))) << 3); }
-__device__ __forceinline__ int v_at(int dim, int ch) { return dim * PAGE + ((ch ^ (dim & 7)) << 3); }
+__device__ __forceinline__ int v_at(int dim, int ch) { return dim * PAGE + ((ch ^ ((dim >> 1) & 7)) << 3); }
 
 template <int D>
 __global__ void __launch_bounds__(LNT, 2)
@@ -461,7 +476,7 @@ attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, c
                  int Hq, int Hkv, int pages, int target, float scale_log2) {
   constexpr int KS = D / 16, DC = D / 32;              // k-steps of the scores, 32-wide blocks of the output
   constexpr int CHUNKS = PAGE * D / 16;                // 16-byte chunks of codes in a page, each of K and V
-  __shared__ __attribute__((aligned(16))) bf16_t s_k[2][PAGE * D], s_v[2][PAGE * D];
+  __shared__ __attribute__((aligned(16))) bf16_t s_k[4][PAGE * D], s_v[4][PAGE * D];
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 31, h = lane >> 5;
   // kv head = workgroup mod Hkv: with 8 of them each XCD's L2 serves one head's pages
@@ -482,6 +497,8 @@ attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, c
     const bf16_t* qp = q + ((size_t)(tok0 + row / G) * Hq + (size_t)hk * G + row % G) * D + 8 * h;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * s);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) arrived(qf[s]);
   }
   f32x16_t o[DC];
 #pragma unroll
@@ -494,10 +511,10 @@ attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, c
   const int p0 = (int)((long long)npages * sh.part / ns), p1 = (int)((long long)npages * (sh.part + 1) / ns);
   int ids = 0;                                         // lane i: one of the next 64 pages, and its scales
   float kss = 0.f, vss = 0.f;
-  uint4 kr = make_uint4(0, 0, 0, 0), vr = kr;          // the next page's codes, and what goes with them
-  float ks = 0.f, vs = 0.f;
-  bool bad = false;
-  auto fetch = [&](int p) {
+  uint4 kr[2], vr[2];                                  // the next two pages' codes, and what goes with them
+  float ks[2], vs[2];
+  bool bad[2] = {false, false};                        // not a page of the cache: its keys count as masked
+  auto fetch = [&](int z, int p) __attribute__((always_inline)) {
     const int at = (p - p0) & 63;
     if (at == 0) {
       ids = table[(size_t)b * W + min(p + lane, npages - 1)];
@@ -506,55 +523,45 @@ attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, c
       vss = vscale[x];
     }
     const int id = __builtin_amdgcn_readlane(ids, at);
-    ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), at));
-    vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vss), at));
-    bad = id < 0 || id >= pages;
-    const size_t ph = ((size_t)(bad ? 0 : id) * Hkv + hk) * (PAGE * D);
+    ks[z] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), at));
+    vs[z] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vss), at));
+    bad[z] = id < 0 || id >= pages;
+    const size_t ph = ((size_t)(bad[z] ? 0 : id) * Hkv + hk) * (PAGE * D);
     if (t < CHUNKS) {
-      kr = *reinterpret_cast<const uint4*>(kc + ph + 16 * t);
-      vr = *reinterpret_cast<const uint4*>(vc + ph + 16 * t);
+      kr[z] = *reinterpret_cast<const uint4*>(kc + ph + 16 * t);
+      vr[z] = *reinterpret_cast<const uint4*>(vc + ph + 16 * t);
     }
   };
-  auto stage = [&](int buf, int p) {
+  auto stage = [&](int z, int buf, int p) __attribute__((always_inline)) {
     if (t < CHUNKS) {
       const int kt = t / (D / 16), kch = t % (D / 16) * 2;
-      *reinterpret_cast<bf16x8_t*>(&s_k[buf][k_at<D>(kt, kch)]) = widen(kr.x, kr.y, ks);
-      *reinterpret_cast<bf16x8_t*>(&s_k[buf][k_at<D>(kt, kch + 1)]) = widen(kr.z, kr.w, ks);
-      const int dim = t / (PAGE / 16), qk = t % (PAGE / 16), live = bad ? 0 : L - p * PAGE;
+      *reinterpret_cast<bf16x8_t*>(&s_k[buf][k_at<D>(kt, kch)]) = widen(kr[z].x, kr[z].y, ks[z]);
+      *reinterpret_cast<bf16x8_t*>(&s_k[buf][k_at<D>(kt, kch + 1)]) = widen(kr[z].z, kr[z].w, ks[z]);
+      const int dim = t / (PAGE / 16), qk = t % (PAGE / 16), live = bad[z] ? 0 : L - p * PAGE;
+      uint4& v = vr[z];
       if (live < PAGE) {                               // slots never written may hold any code, NaN too
-        vr.x &= live_bytes(16 * qk, live);
-        vr.y &= live_bytes(16 * qk + 4, live);
-        vr.z &= live_bytes(16 * qk + 8, live);
-        vr.w &= live_bytes(16 * qk + 12, live);
+        v.x &= live_bytes(16 * qk, live);
+        v.y &= live_bytes(16 * qk + 4, live);
+        v.z &= live_bytes(16 * qk + 8, live);
+        v.w &= live_bytes(16 * qk + 12, live);
       }
-      *reinterpret_cast<bf16x8_t*>(&s_v[buf][v_at(dim, 2 * qk)]) = widen(vr.x, vr.z, vs);
-      *reinterpret_cast<bf16x8_t*>(&s_v[buf][v_at(dim, 2 * qk + 1)]) = widen(vr.y, vr.w, vs);
+      *reinterpret_cast<bf16x8_t*>(&s_v[buf][v_at(dim, 2 * qk)]) = widen(v.x, v.z, vs[z]);
+      *reinterpret_cast<bf16x8_t*>(&s_v[buf][v_at(dim, 2 * qk + 1)]) = widen(v.y, v.w, vs[z]);
     }
   };
 
-  if (p0 < p1) {
-    fetch(p0);
-    stage(0, p0);
-  }
-  __syncthreads();
-  for (int p = p0; p < p1; ++p) {
-    const int buf = (p - p0) & 1, key0 = p * PAGE;
-    const bool masked = bad;                           // of this page; fetch moves on to the next
-    if (p + 1 < p1) fetch(p + 1);
+  auto page = [&](int p, int buf, bool masked) __attribute__((always_inline)) {
+    const int key0 = p * PAGE;
     if (!idle && key0 < most) {
-      const bool two = key0 + 32 < most;               // some row sees a key of the second half
       const bf16_t* sk = s_k[buf];
       const bf16_t* sv = s_v[buf];
       f32x16_t s0, s1;
 #pragma unroll
       for (int i = 0; i < 16; ++i) s0[i] = 0.f, s1[i] = 0.f;
 #pragma unroll
-      for (int st = 0; st < KS; ++st)
+      for (int st = 0; st < KS; ++st) {
         s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(&sk[k_at<D>(r, 2 * st + h)]), qf[st], s0, 0, 0, 0);
-      if (two) {
-#pragma unroll
-        for (int st = 0; st < KS; ++st)
-          s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(&sk[k_at<D>(32 + r, 2 * st + h)]), qf[st], s1, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(&sk[k_at<D>(32 + r, 2 * st + h)]), qf[st], s1, 0, 0, 0);
       }
       if (masked || key0 + PAGE > least) {
         const int seen = (masked ? 0 : vis - key0) - 4 * h;
@@ -567,10 +574,8 @@ attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, c
       float mx = s0[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s0[i]);
-      if (two) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s1[i]);
-      }
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s1[i]);
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
       const float mt = mx * scale_log2;
       if (__ballot(mt > m + 8.f)) {
@@ -590,15 +595,13 @@ attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, c
         s0[i] = __builtin_amdgcn_exp2f(fmaf(s0[i], scale_log2, -base));
         sum += s0[i];
       }
-      if (two) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s1[i] = __builtin_amdgcn_exp2f(fmaf(s1[i], scale_log2, -base));
-          sum += s1[i];
-        }
+      for (int i = 0; i < 16; ++i) {
+        s1[i] = __builtin_amdgcn_exp2f(fmaf(s1[i], scale_log2, -base));
+        sum += s1[i];
       }
       l += sum;
-      auto pv = [&](const f32x16_t& s, int u) {        // k-step u of the page's four
+      auto pv = [&](const f32x16_t& s, int u) __attribute__((always_inline)) {        // k-step u of the page's four
         bf16x8_t pf;
 #pragma unroll
         for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[8 * (u & 1) + j];
@@ -608,13 +611,41 @@ attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, c
       };
       pv(s0, 0);
       pv(s0, 1);
-      if (two) {
-        pv(s1, 2);
-        pv(s1, 3);
-      }
+      pv(s1, 2);
+      pv(s1, 3);
     }
-    if (p + 1 < p1) stage(buf ^ 1, p + 1);
+  };
+  auto fetch_two = [&](int p) __attribute__((always_inline)) {
+    if (p < p1) fetch(0, p);
+    if (p + 1 < p1) fetch(1, p + 1);
+  };
+  auto stage_two = [&](int p, int buf) __attribute__((always_inline)) {
+    if (p < p1) stage(0, buf, p);
+    if (p + 1 < p1) stage(1, buf + 1, p + 1);
+  };
+  bool now[2];
+  if (p0 < p1) {
+    fetch_two(p0);
+    stage_two(p0, 0);
+  }
+  now[0] = bad[0], now[1] = bad[1];
+  fetch_two(p0 + 2);
+  __syncthreads();
+  auto two = [&](int p, auto buf) __attribute__((always_inline)) {
+    constexpr int B0 = decltype(buf)::value;
+    page(p, B0, now[0]);
+    const bool second = now[1];
+    if (p + 2 < p1) {
+      stage_two(p + 2, B0 ^ 2);
+      now[0] = bad[0], now[1] = bad[1];
+      fetch_two(p + 4);
+    }
+    if (p + 1 < p1) page(p + 1, B0 + 1, second);
     __syncthreads();
+  };
+  for (int p = p0; p < p1; p += 4) {
+    two(p, std::integral_constant<int, 0>());
+    if (p + 2 < p1) two(p + 2, std::integral_constant<int, 2>());
   }
 
   // lane (r, h) holds dims 32 dc + 8 j + 4 h .. + 4 of its row
