@@ -114,7 +114,7 @@ __device__ __forceinline__ int wave_scan(int v) {
 // fit 31 bits.
 template <int ROWS, int SMALLEST>
 __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const int* __restrict__ kv_lens, int N, int B, int W,
-                                            int G, int target, int above, int upto, int me) {
+                                            int G, int target, int above, int upto, int me, int Hkv) {
   const int lane = threadIdx.x & 63, per = (B + 63) / 64;
   int tiles = 0, np = 0;
   auto size = [&](int b) {
@@ -147,10 +147,12 @@ __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const in
     split += ns > 1 ? tiles * ns : 0;
   }
   const int end = wave_scan(sum), at = end - sum, slot = wave_scan(split) - split;
-  me = __builtin_amdgcn_readlane(end, 63) - 1 - me;
+  const int all = __builtin_amdgcn_readlane(end, 63);
+  me = all - 1 - me;
   const unsigned long long owner = __ballot(me >= at && me < end);
   Share sh = {0, 0, 0, 0, 0};
-  if (owner == 0) return sh;
+  // requests that overlap may have more parts than the launch: then none is worked on, so that none waits in a counter
+  if (owner == 0 || (long long)all * Hkv > gridDim.x) return sh;
   const int who = __ffsll((long long)owner) - 1;
   int x = me - __builtin_amdgcn_readlane(at, who);
   sh.b = who * per;
@@ -159,6 +161,7 @@ __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const in
     sh.ns = __builtin_amdgcn_readlane(parts(np), who);
   } else {
     for (;; ++sh.b) {          // ends inside the lane's requests: x is below their sum
+      if (sh.b >= B) return Share{0, 0, 0, 0, 0};
       size(sh.b);
       sh.ns = parts(np);
       if (x < tiles * sh.ns) break;
@@ -171,6 +174,8 @@ __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const in
   sh.tile = __builtin_amdgcn_readfirstlane(x / sh.ns);
   sh.part = __builtin_amdgcn_readfirstlane(x % sh.ns);
   sh.slot = __builtin_amdgcn_readfirstlane(sh.slot) + sh.tile * sh.ns;
+  // split tiles have at most `goal` whole chunks and one part more each: never past the workspace
+  if (sh.ns > 1 && (sh.slot < 0 || sh.slot + sh.ns > 2 * target)) sh.ns = 0;
   return sh;
 }
 
@@ -192,7 +197,7 @@ attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const 
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 15, a = lane >> 4;
   const int G = Hq / Hkv, hk = blockIdx.x % Hkv;
-  const Share sh = find_share<TILE, MIN_CHUNK>(cu, kv_lens, N, B, W, G, target, 0, upto, blockIdx.x / Hkv);
+  const Share sh = find_share<TILE, MIN_CHUNK>(cu, kv_lens, N, B, W, G, target, 0, upto, blockIdx.x / Hkv, Hkv);
   if (sh.ns == 0) return;
   const int b = sh.b, row0 = sh.tile * TILE, ns = sh.ns;
   const int tok0 = min(max(cu[b], 0), N), n = min(cu[b + 1], N) - tok0, rows = n * G;
@@ -481,7 +486,7 @@ attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, c
   const int r = lane & 31, h = lane >> 5;
   // kv head = workgroup mod Hkv: with 8 of them each XCD's L2 serves one head's pages
   const int G = Hq / Hkv, hk = blockIdx.x % Hkv;
-  const Share sh = find_share<LTILE, LMIN_CHUNK>(cu, kv_lens, N, B, W, G, target, SHORT_ROWS, INT_MAX, blockIdx.x / Hkv);
+  const Share sh = find_share<LTILE, LMIN_CHUNK>(cu, kv_lens, N, B, W, G, target, SHORT_ROWS, INT_MAX, blockIdx.x / Hkv, Hkv);
   if (sh.ns == 0) return;
   const int b = sh.b, ns = sh.ns, tile0 = sh.tile * LTILE, row0 = tile0 + 32 * w;
   const int tok0 = min(max(cu[b], 0), N), n = min(cu[b + 1], N) - tok0, rows = n * G;

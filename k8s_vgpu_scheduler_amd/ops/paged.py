@@ -27,6 +27,7 @@ from k8s_vgpu_scheduler_amd import ops
 
 PAGE = 64            # tokens of a page (csrc/ops/paged.h)
 MAX_ROWS = 1024      # requests of one call
+MAX_KV_HEADS = 256   # of paged_attention (csrc/ops/paged_attn.hip MAX_HKV)
 
 
 _I32, _I64, _F32, _BF16, _FP8 = torch.int32, torch.int64, torch.float32, torch.bfloat16, torch.float8_e4m3fn
@@ -61,6 +62,8 @@ def _launch(idx: int, name: str, fn, *args):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     if rc == -2:
         raise ValueError(f"{name}: the workspace is too small for this call")
+    if rc == -1:
+        raise ValueError(f"{name}: sizes past the kernels' 32-bit indices")
     ops._check(rc, name)
 
 
@@ -236,10 +239,10 @@ def paged_attention_workspace(n_tokens: int, rows: int, n_q_heads: int, n_kv_hea
     """Workspace of ``paged_attention`` for steps of up to ``n_tokens`` tokens and ``rows`` requests: room for the parts
     that a long request is split into, and counters that every call leaves at zero.  Calls that may run at once (two
     streams, two captured graphs replayed side by side) need one each."""
-    if n_tokens < 0 or not 0 < rows <= MAX_ROWS or n_kv_heads < 1 or n_q_heads < 1 or n_q_heads % n_kv_heads \
-            or head_dim not in (64, 128):
+    if not 0 <= n_tokens < 2**31 or not 0 < rows <= MAX_ROWS or not 0 < n_kv_heads <= MAX_KV_HEADS or n_q_heads < 1 \
+            or n_q_heads % n_kv_heads or head_dim not in (64, 128):
         raise ValueError(f"paged_attention_workspace: {n_tokens} tokens of {rows} requests, {n_q_heads} / {n_kv_heads} "
-                         f"heads of {head_dim} (64 or 128)")
+                         f"(at most {MAX_KV_HEADS}) heads of {head_dim} (64 or 128)")
     zeroed = ctypes.c_longlong(0)
     with torch.cuda.device(device):
         floats = ops.lib().mivgpu_paged_attention_work(n_tokens, n_q_heads, n_kv_heads, ctypes.byref(zeroed))
@@ -259,10 +262,14 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, table: torch.Tensor, cu_q: 
     new tokens of a request, if known (1 in a decode step).  ``work`` from ``paged_attention_workspace``."""
     name = "paged_attention"
     pages, specs = _cache_specs(cache, name, n_q_heads, n_kv_heads, head_dim)
+    if n_kv_heads > MAX_KV_HEADS:
+        raise ValueError(f"{name}: {n_kv_heads} kv heads (at most {MAX_KV_HEADS})")
+    if q.dim() != 3 or not 0 < scale < math.inf:
+        raise ValueError(f"{name}: q must be [N, {n_q_heads}, {head_dim}], got {list(q.shape)}, and scale positive, got {scale}")
     N = q.shape[0]
     if table.dim() != 2 or not 0 < table.shape[0] <= MAX_ROWS or table.shape[1] < 1 or table.shape[1] * PAGE > 2**31 - 1:
         raise ValueError(f"{name}: table must be [B <= {MAX_ROWS}, W], got {list(table.shape)}")
-    if max_new is not None and max_new < 0:
+    if max_new is not None and not 0 <= max_new < 2**31:
         raise ValueError(f"{name}: max_new {max_new}")
     B, W = table.shape
     if out is None:

@@ -118,11 +118,20 @@ def attn_args(**bad):
     {}, dict(q=bf(3, 4, 128).float()), dict(q=bf(3, 5, 128)), dict(q=bf(4, 3, 128).transpose(0, 1)),
     dict(table=i32(2)), dict(table=i32(0, 3)), dict(table=i32(2, 0)), dict(table=i32(1025, 1)), dict(cu_q=i32(2)),
     dict(cu_q=i32(3).long()), dict(kv_lens=i32(3)), dict(out=bf(3, 511)), dict(out=bf(2, 512)), dict(n_q_heads=5),
-    dict(head_dim=64), dict(max_new=-1), dict(cache=cache(4, 4)),
+    dict(head_dim=64), dict(max_new=-1), dict(cache=cache(4, 4)), dict(q=bf(3, 512)), dict(scale=0.0), dict(scale=-0.1),
+    dict(scale=math.nan), dict(scale=math.inf), dict(max_new=2**31),
+    dict(q=bf(1, 257, 64), cache=cache(1, 257, 64), n_q_heads=257, n_kv_heads=257, head_dim=64, out=bf(1, 257 * 64)),
 ])
 def test_attention_refuses(bad):
     with pytest.raises(ValueError, match="paged_attention"):
         ops.paged_attention(**attn_args(**bad))
+
+
+@pytest.mark.parametrize("args", [(-1, 1, 4, 2, 128), (2**31, 1, 4, 2, 128), (1, 0, 4, 2, 128), (1, 1025, 4, 2, 128), (1, 1, 5, 2, 128),
+                                  (1, 1, 4, 0, 128), (1, 1, 257, 257, 64), (1, 1, 4, 2, 96)])
+def test_attention_workspace_refuses(args):
+    with pytest.raises(ValueError, match="paged_attention_workspace"):
+        ops.paged_attention_workspace(*args, device="cpu")
 
 
 def sample_args(**bad):

@@ -457,6 +457,46 @@ def test_attention_equal_scores(ops):
     check_attention(ops, q * 0, cache, table, cu, kv, 4, 2, 128)
 
 
+def test_attention_workspace_too_small(ops):
+    """Room for few rows does not do for many; nothing is launched."""
+    q, cache, table, cu, kv = attention_case(ops, [0], [300], 4, 2, 128)
+    few = ops.paged_attention_workspace(1, 1, 4, 2, 128)
+    for work in (few, few[:100]):
+        with pytest.raises(ValueError, match="workspace"):
+            ops.paged_attention(q.cuda(), cache, dev(table), dev(cu), dev(kv), 4, 2, 128, 0.1, work=work)
+    for bad in (few.double(), few[::2], few[1:], few.view(1, -1), few.cpu()):
+        with pytest.raises(ValueError, match="paged_attention"):
+            ops.paged_attention(q.cuda(), cache, dev(table), dev(cu), dev(kv), 4, 2, 128, 0.1, work=bad)
+
+
+def test_attention_one_workspace_for_all(ops):
+    """Steps of other sizes, heads and kinds in turn on one workspace: each finds it as the first did."""
+    work = ops.paged_attention_workspace(1024, 64, 32, 1, 128)
+    for name in list(ATTNS) + ["single", "chunk beside decode", "prompts", "group of sixteen"]:
+        old, new, hq, hkv, d = ATTNS[name]
+        q, cache, table, cu, kv = attention_case(ops, old, new, hq, hkv, d)
+        check_attention(ops, q, cache, table, cu, kv, hq, hkv, d, work=work)
+    assert (work[:1024] == 0).all()
+
+
+def test_attention_more_new_tokens_than_said(ops):
+    q, cache, table, cu, kv = attention_case(ops, [500, 77, 0], [130, 1, 70], 8, 2, 128)
+    for said in (0, 1, 16, 17, 130):
+        check_attention(ops, q, cache, table, cu, kv, 8, 2, 128, max_new=said)
+
+
+@pytest.mark.parametrize("new", [3, 90])
+def test_attention_overlapping_requests_stay_in_bounds(ops, new):
+    """Rows that several requests claim have no answer, but nothing outside them is touched and the next call is right."""
+    q, cache, table, cu, kv = attention_case(ops, [2000] * 6, [new] * 6, 4, 2, 128)
+    work = ops.paged_attention_workspace(6 * new, 6, 4, 2, 128)
+    out = torch.full((6 * new + 3, 512), 5.0, dtype=torch.bfloat16, device="cuda")
+    n = 6 * new
+    ops.paged_attention(q.cuda(), cache, dev(table), dev([0, n, 0, n, 0, n, n]), dev(kv), 4, 2, 128, 0.1, out=out, work=work)
+    assert (out[n:] == 5.0).all()
+    check_attention(ops, q, cache, table, cu, kv, 4, 2, 128, work=work)
+
+
 def test_attention_nothing(ops):
     cache = ops.paged_kv_cache(1, 1, 64)
     out = ops.paged_attention(torch.empty(0, 1, 64, dtype=torch.bfloat16, device="cuda"), cache, dev([[0]]), dev([0, 0]),
