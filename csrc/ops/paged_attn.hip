@@ -45,8 +45,8 @@ constexpr int LNT = 512, LWAVES = 8, LTILE = 32 * LWAVES;
 constexpr int LMIN_CHUNK = 8;
 
 // A call aims at as many workgroups as are resident (two of the short ones with D = 64 a CU, otherwise one), over all kv
-// heads, and with that bounds the slots of the workspace: with t parts aimed at a kv head a split tile of np pages gets at most np / chunk + 1 <= 2 np / chunk parts, which
-// add up to at most 2 t.
+// heads, and with that bounds the slots of the workspace: with t parts aimed at a kv head a split tile of np pages gets at
+// most np / chunk + 1 <= 2 np / chunk parts, which add up to at most 2 t.
 constexpr int MAX_CUS = 256, MAX_HKV = 256;
 constexpr int SHORT_SLOTS = 2 * 2 * MAX_CUS, LONG_SLOTS = 2 * MAX_CUS;
 
@@ -653,60 +653,83 @@ attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, c
     if (p + 2 < p1) two(p + 2, std::integral_constant<int, 2>());
   }
 
-  // lane (r, h) holds dims 32 dc + 8 j + 4 h .. + 4 of its row
+  // Parts of a tile: a wave's rows are joined with the same wave's of the other parts, without the rest of the
+  // workgroup.  All but the last to arrive leave (m, l) and O, in the order of their registers, and count themselves
+  // done; the last has its own at hand and waits for the others, which are past their arrival and wait for nothing.  It
+  // adds the parts in their order, whoever came last.  (Two parts of 39 pages each a tile, 32 / 8 heads: 90 us; with all
+  // parts stored in rows of the output, counted once a workgroup and read again 113.)
+  if (idle) return;
   l += __shfl_xor(l, 32, 64);
-  const size_t slot0 = (size_t)sh.slot * Hkv + hk, mine = (slot0 + (size_t)sh.part * Hkv) * LTILE + 32 * w + r;
+  if (ns > 1) {
+    const size_t slot0 = (size_t)sh.slot * Hkv + hk;
+    const auto at = [&](int part) { return (slot0 + (size_t)part * Hkv) * (LNT / 64) + w; };
+    int *arrived_at = counters + at(0), *done_at = counters + at(1), came = 0;
+    if (lane == 0) came = __hip_atomic_fetch_add(arrived_at, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__builtin_amdgcn_readfirstlane(came) != ns - 1) {
+      float* to = part_o + (at(sh.part) * (D / 4) * 64 + lane) * 2;
+#pragma unroll
+      for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) put2(to + (8 * dc + i / 2) * 128, o[dc][i], o[dc][i + 1]);
+      if (h == 0) put2(part_ml + (at(sh.part) * 32 + r) * 2, m, l);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // as in attn_kernel
+      if (lane == 0) __hip_atomic_fetch_add(done_at, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      return;
+    }
+    while (__builtin_amdgcn_readfirstlane(__hip_atomic_load(done_at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) != ns - 1)
+      __builtin_amdgcn_s_sleep(1);
+    asm volatile("" ::: "memory");
+    if (lane == 0) {
+      __hip_atomic_store(arrived_at, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(done_at, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    float top = m;
+    for (int i = 0; i < ns; ++i)
+      if (i != sh.part) top = fmaxf(top, get2(part_ml + (at(i) * 32 + r) * 2).x);
+    const float base = top == -INFINITY ? 0.f : top;
+    f32x16_t mine[DC];
+    float ll = 0.f;
+#pragma unroll
+    for (int dc = 0; dc < DC; ++dc) {
+      mine[dc] = o[dc];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dc][i] = 0.f;
+    }
+    for (int i = 0; i < ns; ++i) {
+      f32x16_t x[DC];
+      float2 e = {m, l};
+      if (i != sh.part) {
+        e = get2(part_ml + (at(i) * 32 + r) * 2);
+        const float* from = part_o + (at(i) * (D / 4) * 64 + lane) * 2;
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            const float2 y = get2(from + (8 * dc + j / 2) * 128);
+            x[dc][j] = y.x;
+            x[dc][j + 1] = y.y;
+          }
+      } else {
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc) x[dc] = mine[dc];
+      }
+      const float f = __builtin_amdgcn_exp2f(e.x - base);
+      ll += e.y * f;
+#pragma unroll
+      for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[dc][j] += x[dc][j] * f;
+    }
+    l = ll;
+  }
+  // lane (r, h) holds dims 32 dc + 8 j + 4 h .. + 4 of its row
   if (row0 + r < rows) {
 #pragma unroll
     for (int dc = 0; dc < DC; ++dc)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int d = 32 * dc + 8 * j + 4 * h;
-        const f32x4_t x = {o[dc][4 * j], o[dc][4 * j + 1], o[dc][4 * j + 2], o[dc][4 * j + 3]};
-        if (ns == 1) {
-          store_row(out, x, l, row, tok0, G, Hq, hk, D, d);
-        } else {
-          put2(part_o + mine * D + d, x[0], x[1]);
-          put2(part_o + mine * D + d + 2, x[2], x[3]);
-        }
-      }
-    if (ns > 1 && h == 0) put2(part_ml + mine * 2, m, l);
-  }
-  if (ns == 1) return;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // as in attn_kernel
-  __syncthreads();
-  int* s_last = reinterpret_cast<int*>(s_k);
-  if (t == 0) *s_last = __hip_atomic_fetch_add(&counters[slot0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ns - 1;
-  __syncthreads();
-  if (!*s_last) return;
-  if (t == 0) __hip_atomic_store(&counters[slot0], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  const int live = min(LTILE, rows - tile0);
-  for (int x = t; x < live * (D / 4); x += LNT) {
-    const int rr = x / (D / 4), d = x % (D / 4) * 4;
-    float mm = -INFINITY, ll = 0.f;
-    f32x4_t oo = {0.f, 0.f, 0.f, 0.f};
-    constexpr int AHEAD = 4;                           // loads in flight
-    for (int i0 = 0; i0 < ns; i0 += AHEAD) {
-      float2 ml[AHEAD], x01[AHEAD], x23[AHEAD];
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        const size_t at = (slot0 + (size_t)min(i0 + j, ns - 1) * Hkv) * LTILE + rr;
-        ml[j] = get2(part_ml + at * 2);
-        x01[j] = get2(part_o + at * D + d);
-        x23[j] = get2(part_o + at * D + d + 2);
-      }
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        if (i0 + j < ns) {
-          const float mnew = fmaxf(mm, ml[j].x), base = mnew == -INFINITY ? 0.f : mnew;
-          const float f0 = __builtin_amdgcn_exp2f(mm - base), f1 = __builtin_amdgcn_exp2f(ml[j].x - base);
-          mm = mnew;
-          ll = ll * f0 + ml[j].y * f1;
-          oo = oo * f0 + f32x4_t{x01[j].x, x01[j].y, x23[j].x, x23[j].y} * f1;
-        }
-      }
-    }
-    store_row(out, oo, ll, tile0 + rr, tok0, G, Hq, hk, D, d);
+      for (int j = 0; j < 4; ++j)
+        store_row(out, f32x4_t{o[dc][4 * j], o[dc][4 * j + 1], o[dc][4 * j + 2], o[dc][4 * j + 3]}, l, row, tok0, G, Hq, hk,
+                  D, 32 * dc + 8 * j + 4 * h);
   }
 }
 
@@ -722,7 +745,7 @@ static int all_cus() {
 
 // The workspace, for any head size: counters (zero before the first call, left zero), then (m, l) and O of the short
 // and, where a call has more rows than SHORT_ROWS, of the long tiles' parts.
-constexpr long long ZEROED = SHORT_SLOTS + LONG_SLOTS;
+constexpr long long ZEROED = SHORT_SLOTS + LONG_SLOTS * (LNT / 64);
 constexpr long long SHORT_FLOATS = (long long)SHORT_SLOTS * TILE * (2 + 128);
 constexpr long long LONG_FLOATS = (long long)LONG_SLOTS * LTILE * (2 + 128);
 
