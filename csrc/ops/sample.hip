@@ -71,12 +71,20 @@ struct Row {
   __device__ bool whole(int turn) const { return 8 * (from + 64 * turn) >= lead && 8 * (from + 64 * turn + 64) <= V + lead; }
   __device__ int vec(int turn) const { return from + 64 * turn + (int)(threadIdx.x & 63); }
   __device__ __forceinline__ uint4 load(int turn) const { return at[min(vec(turn), vecs - 1)]; }
+  // the lane's first vectors, asked for ahead of a look at the row
+  struct Batch { uint4 v[BATCH]; };
+  __device__ __forceinline__ Batch first() const {
+    Batch y;
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) y.v[j] = load(j);
+    return y;
+  }
   // f(bins of the lane's vector, turn) for all turns, the next batch on its way; before(batch) ahead of each
   template <class F, class G>
-  __device__ __forceinline__ void each(int turns, F f, G before) const {
+  __device__ __forceinline__ void each(const Batch& begin, int turns, F f, G before) const {
     uint4 x[BATCH], y[BATCH];
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) y[j] = load(j);
+    for (int j = 0; j < BATCH; ++j) y[j] = begin.v[j];
     for (int i = 0; i < turns; i += BATCH) {
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) x[j] = y[j];
@@ -91,7 +99,9 @@ struct Row {
     }
   }
   template <class F>
-  __device__ __forceinline__ void each(int turns, F f) const { each(turns, f, [](int) {}); }
+  __device__ __forceinline__ void each(const Batch& begin, int turns, F f) const { each(begin, turns, f, [](int) {}); }
+  template <class F>
+  __device__ __forceinline__ void each(int turns, F f) const { each(first(), turns, f); }
   // bins of a turn's vector; what is not the row's reads as masked
   __device__ __forceinline__ uint4 bins(uint4 x, int turn) const {
     x = make_uint4(bins_of(x.x), bins_of(x.y), bins_of(x.z), bins_of(x.w));
@@ -168,6 +178,7 @@ sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, int turns,
   __shared__ Shared sh;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), b = blockIdx.x;
   const Row row(logits + (size_t)b * ld, V, turns, w);
+  Row::Batch begin = row.first();
   const float T = temperature != nullptr ? temperature[b] : 1.f;
   if (t == 0) {
     sh.first = BINS;
@@ -195,7 +206,7 @@ sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, int turns,
 
   if (!(T > 0.f)) {                // greedy
     uint32_t lo = 0xffffffffu, hi = 0;
-    row.each(turns, [&](const uint4& x, int) {
+    row.each(begin, turns, [&](const uint4& x, int) {
       lo = min2(lo, min2(min2(x.x, x.y), min2(x.z, x.w)));
       hi = max2(hi, max2(max2(x.x, x.y), max2(x.z, x.w)));
     });
@@ -251,7 +262,7 @@ sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, int turns,
     auto add = [&](uint32_t bin) { atomicAdd(&hist[bin >> 1], 1u + (bin & 1) * 0xffffu); };
     int masked = 0;
     row.each(
-        turns,
+        begin, turns,
         [&](const uint4& x, int) {
           const uint32_t top = max2(max2(x.x, x.y), max2(x.z, x.w));
           const bool some = (top & 0xffffu) >= (uint32_t)BIN_MINUS_INF || (top >> 16) >= (uint32_t)BIN_MINUS_INF;
@@ -349,6 +360,7 @@ sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, int turns,
   }
 
   // ---- from here on every wave does the same
+  begin = row.first();                           // for the last look
   const int total = sh.before_c[UNITS];
   // weight of the first n >= 1 tokens in order
   auto weight_to = [&](int n) {
@@ -418,7 +430,7 @@ sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, int turns,
     return mask;
   };
   int n = 0;
-  row.each(turns, [&](const uint4& x, int i) {
+  row.each(begin, turns, [&](const uint4& x, int i) {
     uint32_t far = 0x00010001u;                  // 0 in a half where some token matches
 #pragma unroll
     for (int j = 0; j < 4; ++j) far = min2(far, word_of(x, j) ^ pattern);
