@@ -6,12 +6,14 @@
 // in one pass over the pages with the running maximum m and sum (fp32).
 //
 // The rows of one kv head's G query heads are flattened (row = token * G + head) and cut into tiles: of 16 rows where
-// a request brings at most SHORT_ROWS of them (decode, a few tokens), of 256 in the others (chunks, prompts); a kernel
-// for each kind.  A tile's pages are split over as many workgroups as keep the chip evenly busy: every workgroup scans
-// the requests' lengths (at most 1024: a few a lane) and takes its share of all tiles' pages, so that one long request
-// among short ones is cut into more parts and nothing is planned on the host.  The parts of a tile leave their
-// (m, l, O) in the workspace, and the last one to arrive (a counter that it sets back to zero) joins them in the order
-// of the parts, so that a call's bits do not depend on who that is.
+// a request brings at most SHORT_ROWS of them (decode, a few tokens), of 256 in the others (chunks, prompts).  Both
+// kinds of workgroups are in one launch, so that the short ones' waits for memory lie beside the long ones' products (a
+// chunk of 855 tokens beside seven decoding requests: 80 us; in a launch each 90).
+// A tile's pages are split over as many workgroups as keep the chip evenly busy: every workgroup scans the requests'
+// lengths (at most 1024: a few a lane) and takes its share of all tiles' pages, so that one long request among short
+// ones is cut into more parts and nothing is planned on the host.  The parts of a tile leave their (m, l, O) in the
+// workspace, and the last one to arrive (a counter that it sets back to zero) joins them in the order of the parts, so
+// that a call's bits do not depend on who that is.
 //
 // Tiles of 16: the eight waves of a workgroup take every eighth page and join in LDS.  Per page of 64 keys a wave
 // computes, with 16x16x32 bf16 MFMAs,
@@ -114,7 +116,7 @@ __device__ __forceinline__ int wave_scan(int v) {
 // fit 31 bits.
 template <int ROWS, int SMALLEST>
 __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const int* __restrict__ kv_lens, int N, int B, int W,
-                                            int G, int target, int above, int upto, int me, int Hkv) {
+                                            int G, int target, int above, int upto, int me, int Hkv, unsigned grid) {
   const int lane = threadIdx.x & 63, per = (B + 63) / 64;
   int tiles = 0, np = 0;
   auto size = [&](int b) {
@@ -152,7 +154,7 @@ __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const in
   const unsigned long long owner = __ballot(me >= at && me < end);
   Share sh = {0, 0, 0, 0, 0};
   // requests that overlap may have more parts than the launch: then none is worked on, so that none waits in a counter
-  if (owner == 0 || (long long)all * Hkv > gridDim.x) return sh;
+  if (owner == 0 || (long long)all * Hkv > grid) return sh;
   const int who = __ffsll((long long)owner) - 1;
   int x = me - __builtin_amdgcn_readlane(at, who);
   sh.b = who * per;
@@ -179,25 +181,58 @@ __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const in
   return sh;
 }
 
+// What both kinds of workgroups are called with
+struct Call {
+  const bf16_t* __restrict__ q;
+  const uint8_t *__restrict__ kc, *__restrict__ vc;
+  const float *__restrict__ kscale, *__restrict__ vscale;
+  const int *__restrict__ table, *__restrict__ cu, *__restrict__ kv_lens;
+  bf16_t* __restrict__ out;
+  int N, B, W, Hq, Hkv, pages;
+  float scale_log2;
+};
+// Of one kind: its workspace, the parts it aims at for each kv head, and its workgroups
+struct Work {
+  int* __restrict__ counters;
+  float *__restrict__ part_ml, *__restrict__ part_o;
+  int target;
+  unsigned grid;
+};
+#define MIVGPU_PATTN_ARGS                                                                                             \
+  const bf16_t* __restrict__ q = c.q;                                                                                 \
+  const uint8_t *__restrict__ kc = c.kc, *__restrict__ vc = c.vc;                                                     \
+  const float *__restrict__ kscale = c.kscale, *__restrict__ vscale = c.vscale;                                       \
+  const int *__restrict__ table = c.table, *__restrict__ cu = c.cu, *__restrict__ kv_lens = c.kv_lens;                \
+  bf16_t* __restrict__ out = c.out;                                                                                   \
+  int* __restrict__ counters = k.counters;                                                                            \
+  float *__restrict__ part_ml = k.part_ml, *__restrict__ part_o = k.part_o;                                           \
+  const int N = c.N, B = c.B, W = c.W, Hq = c.Hq, Hkv = c.Hkv, pages = c.pages, target = k.target;                    \
+  const float scale_log2 = c.scale_log2
+
 template <int D>
-__global__ void __launch_bounds__(NT, D == 64 ? 4 : 2)
-attn_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
-            const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ table,
-            const int* __restrict__ cu, const int* __restrict__ kv_lens, bf16_t* __restrict__ out,
-            int* __restrict__ counters, float* __restrict__ part_ml, float* __restrict__ part_o, int N, int B, int W,
-            int Hq, int Hkv, int pages, int target, int upto, float scale_log2) {
+struct ShortLds {
+  float m[WAVES][TILE], l[WAVES][TILE];
+  int last;
+  // the waves' O; later the (m, l) of a tile's parts and what groups of threads make of them
+  static constexpr int O_BYTES = WAVES * TILE * (JOIN + 4) * 4, JOIN_BYTES = MAX_PARTS * TILE * 8 + NT * 20;
+  __attribute__((aligned(16))) char raw[O_BYTES > JOIN_BYTES ? O_BYTES : JOIN_BYTES];
+};
+
+// upto: the most rows of a request that the short tiles take
+template <int D>
+__device__ __forceinline__ void short_part(const Call& c, const Work& k, int upto, unsigned block, ShortLds<D>& lds) {
+  MIVGPU_PATTN_ARGS;
   constexpr int KU = D / 64;              // 16-byte chunks of a K row per lane
   constexpr int DT = D / 16;              // output tiles
-  __shared__ float s_m[WAVES][TILE], s_l[WAVES][TILE];
-  // the waves' O; later the (m, l) of a tile's parts and what groups of threads make of them
-  constexpr int O_BYTES = WAVES * TILE * (JOIN + 4) * 4, JOIN_BYTES = MAX_PARTS * TILE * 8 + NT * 20;
-  __shared__ __attribute__((aligned(16))) char s_raw[O_BYTES > JOIN_BYTES ? O_BYTES : JOIN_BYTES];
+  auto& s_m = lds.m;
+  auto& s_l = lds.l;
+  auto& s_raw = lds.raw;
+  int& s_last = lds.last;
   float(*s_o)[TILE][JOIN + 4] = reinterpret_cast<float(*)[TILE][JOIN + 4]>(s_raw);
-  __shared__ int s_last;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 15, a = lane >> 4;
-  const int G = Hq / Hkv, hk = blockIdx.x % Hkv;
-  const Share sh = find_share<TILE, MIN_CHUNK>(cu, kv_lens, N, B, W, G, target, 0, upto, blockIdx.x / Hkv, Hkv);
+  const int G = Hq / Hkv, hk = block % Hkv;
+  const Share sh = find_share<TILE, MIN_CHUNK>(cu, kv_lens, N, B, W, G, target, 0, upto, block / Hkv, Hkv, k.grid);
   if (sh.ns == 0) return;
   const int b = sh.b, row0 = sh.tile * TILE, ns = sh.ns;
   const int tok0 = min(max(cu[b], 0), N), n = min(cu[b + 1], N) - tok0, rows = n * G;
@@ -473,20 +508,16 @@ __device__ __forceinline__ int k_at(int row, int ch) { return row * D + ((ch ^ (
 __device__ __forceinline__ int v_at(int dim, int ch) { return dim * PAGE + ((ch ^ ((dim >> 1) & 7)) << 3); }
 
 template <int D>
-__global__ void __launch_bounds__(LNT, 2)
-attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
-                 const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ table,
-                 const int* __restrict__ cu, const int* __restrict__ kv_lens, bf16_t* __restrict__ out,
-                 int* __restrict__ counters, float* __restrict__ part_ml, float* __restrict__ part_o, int N, int B, int W,
-                 int Hq, int Hkv, int pages, int target, float scale_log2) {
+__device__ __forceinline__ void long_part(const Call& c, const Work& k, unsigned block, bf16_t (&s_k)[4][PAGE * D], bf16_t (&s_v)[4][PAGE * D]) {
+  MIVGPU_PATTN_ARGS;
   constexpr int KS = D / 16, DC = D / 32;              // k-steps of the scores, 32-wide blocks of the output
   constexpr int CHUNKS = PAGE * D / 16;                // 16-byte chunks of codes in a page, each of K and V
-  __shared__ __attribute__((aligned(16))) bf16_t s_k[4][PAGE * D], s_v[4][PAGE * D];
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 31, h = lane >> 5;
   // kv head = workgroup mod Hkv: with 8 of them each XCD's L2 serves one head's pages
-  const int G = Hq / Hkv, hk = blockIdx.x % Hkv;
-  const Share sh = find_share<LTILE, LMIN_CHUNK>(cu, kv_lens, N, B, W, G, target, SHORT_ROWS, INT_MAX, blockIdx.x / Hkv, Hkv);
+  const int G = Hq / Hkv, hk = block % Hkv;
+  const Share sh =
+      find_share<LTILE, LMIN_CHUNK>(cu, kv_lens, N, B, W, G, target, SHORT_ROWS, INT_MAX, block / Hkv, Hkv, k.grid);
   if (sh.ns == 0) return;
   const int b = sh.b, ns = sh.ns, tile0 = sh.tile * LTILE, row0 = tile0 + 32 * w;
   const int tok0 = min(max(cu[b], 0), N), n = min(cu[b + 1], N) - tok0, rows = n * G;
@@ -657,7 +688,8 @@ attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, c
   // workgroup.  All but the last to arrive leave (m, l) and O, in the order of their registers, and count themselves
   // done; the last has its own at hand and waits for the others, which are past their arrival and wait for nothing.  It
   // adds the parts in their order, whoever came last.  (Two parts of 39 pages each a tile, 32 / 8 heads: 90 us; with all
-  // parts stored in rows of the output, counted once a workgroup and read again 113.)
+  // parts stored in rows of the output, counted once a workgroup and read again 113.  The short requests in a launch of
+  // their own in both.)
   if (idle) return;
   l += __shfl_xor(l, 32, 64);
   if (ns > 1) {
@@ -733,6 +765,29 @@ attn_long_kernel(const bf16_t* __restrict__ q, const uint8_t* __restrict__ kc, c
   }
 }
 
+#undef MIVGPU_PATTN_ARGS
+
+// All rows in short tiles
+template <int D>
+__global__ void __launch_bounds__(NT, D == 64 ? 4 : 2) attn_kernel(const Call c, const Work k) {
+  __shared__ ShortLds<D> lds;
+  short_part<D>(c, k, INT_MAX, blockIdx.x, lds);
+}
+// The long requests' workgroups, then the short ones': these start where the first leave a CU
+template <int D>
+__global__ void __launch_bounds__(NT, 2) attn_both_kernel(const Call c, const Work longs, const Work shorts) {
+  static_assert(NT == LNT, "one launch");
+  __shared__ __attribute__((aligned(16))) bf16_t s_k[4][PAGE * D], s_v[4][PAGE * D];
+  if (blockIdx.x < longs.grid) {
+    long_part<D>(c, longs, blockIdx.x, s_k, s_v);
+  } else if constexpr (sizeof(ShortLds<D>) <= sizeof(s_k)) {
+    short_part<D>(c, shorts, SHORT_ROWS, blockIdx.x - longs.grid, *reinterpret_cast<ShortLds<D>*>(s_k));
+  } else {
+    __shared__ ShortLds<D> lds;
+    short_part<D>(c, shorts, SHORT_ROWS, blockIdx.x - longs.grid, lds);
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -771,11 +826,6 @@ int mivgpu_paged_attention(const void* q, const void* kc, const void* vc, const 
   // said to be.
   const bool longs = rows > SHORT_ROWS && (max_new < 0 || (long long)max_new * G > SHORT_ROWS);
   if (work == nullptr || floats < ZEROED + SHORT_FLOATS + (longs ? LONG_FLOATS : 0)) return -2;
-  float* sml = work + ZEROED;
-  float* so = sml + SHORT_SLOTS * TILE * 2;
-  float* lml = sml + SHORT_FLOATS;
-  float* lo = lml + LONG_SLOTS * LTILE * 2;
-  const float sl2 = scale * 1.4426950408889634f;
   // Parts: no more than the tiles there can be and `target` on top (each part but a tile's last is a whole chunk), nor
   // than all chunks of all tiles
   auto grid_of = [&](long long tiles, int target, int chunk) {
@@ -790,15 +840,16 @@ int mivgpu_paged_attention(const void* q, const void* kc, const void* vc, const 
   const long long few = rows / (SHORT_ROWS + 1), ltiles = rows / LTILE + (few < some ? few : some);
   const long long parts = grid_of(tiles, target, MIN_CHUNK) * Hkv, lparts = grid_of(ltiles, ltarget, LMIN_CHUNK) * Hkv;
   if (tiles * W > INT_MAX || (longs && ltiles * W > INT_MAX) || parts > INT_MAX || lparts > INT_MAX) return -1;
+  if (longs && parts + lparts > INT_MAX) return -1;
+  const Call c = {(const bf16_t*)q, (const uint8_t*)kc, (const uint8_t*)vc, kscale, vscale, table, cu, kv_lens,
+                  (bf16_t*)out, N, B, W, Hq, Hkv, pages, scale * 1.4426950408889634f};
+  const Work shorts = {(int*)work, work + ZEROED, work + ZEROED + SHORT_SLOTS * TILE * 2, target, (unsigned)parts};
+  float* lml = work + ZEROED + SHORT_FLOATS;
+  const Work more = {(int*)work + SHORT_SLOTS, lml, lml + LONG_SLOTS * LTILE * 2, ltarget, (unsigned)lparts};
 #define MIVGPU_PATTN(DD)                                                                                              \
   do {                                                                                                                \
-    if (longs)                                                                                                        \
-      hipLaunchKernelGGL(attn_long_kernel<DD>, dim3((unsigned)lparts), dim3(LNT), 0, s, (const bf16_t*)q,             \
-                         (const uint8_t*)kc, (const uint8_t*)vc, kscale, vscale, table, cu, kv_lens, (bf16_t*)out,    \
-                         (int*)work + SHORT_SLOTS, lml, lo, N, B, W, Hq, Hkv, pages, ltarget, sl2);                   \
-    hipLaunchKernelGGL(attn_kernel<DD>, dim3((unsigned)parts), dim3(NT), 0, s, (const bf16_t*)q,                      \
-                       (const uint8_t*)kc, (const uint8_t*)vc, kscale, vscale, table, cu, kv_lens, (bf16_t*)out,      \
-                       (int*)work, sml, so, N, B, W, Hq, Hkv, pages, target, longs ? SHORT_ROWS : INT_MAX, sl2);      \
+    if (longs) hipLaunchKernelGGL(attn_both_kernel<DD>, dim3((unsigned)(lparts + parts)), dim3(NT), 0, s, c, more, shorts); \
+    else hipLaunchKernelGGL(attn_kernel<DD>, dim3((unsigned)parts), dim3(NT), 0, s, c, shorts);                       \
   } while (0)
   if (head_dim == 128) MIVGPU_PATTN(128);
   else MIVGPU_PATTN(64);

@@ -344,6 +344,7 @@ ATTNS = {
     "prompt": ([0], [300], 8, 2, 128),
     "prompts": ([0, 0, 64], [65, 128, 191], 4, 4, 64),
     "chunk beside decode": ([500, 77, 0, 200], [130, 1, 40, 1], 8, 2, 128),
+    "chunk beside decode, heads of 64": ([700, 77, 0, 200], [300, 1, 40, 1], 4, 4, 64),
     "rows without tokens": ([10, 50, 0], [0, 2, 0], 4, 2, 128),
     "ragged decode": ([3000, 1, 70, 900, 0, 511, 64, 2100], [1] * 8, 16, 2, 128),
     "long chunk": ([700], [600], 4, 1, 128),
@@ -495,6 +496,18 @@ def test_attention_overlapping_requests_stay_in_bounds(ops, new):
     ops.paged_attention(q.cuda(), cache, dev(table), dev([0, n, 0, n, 0, n, n]), dev(kv), 4, 2, 128, 0.1, out=out, work=work)
     assert (out[n:] == 5.0).all()
     check_attention(ops, q, cache, table, cu, kv, 4, 2, 128, work=work)
+
+
+@pytest.mark.parametrize("name", ["single", "long chunk", "chunk beside decode"])
+def test_attention_same_bits(ops, name):
+    """Whichever part of a tile comes last, a call's result is the same."""
+    old, new, hq, hkv, d = ATTNS[name]
+    q, cache, table, cu, kv = attention_case(ops, old, new, hq, hkv, d)
+    args = (q.cuda(), cache, dev(table), dev(cu), dev(kv), hq, hkv, d, 0.1)
+    work = ops.paged_attention_workspace(len(q), len(kv), hq, hkv, d)
+    want = ops.paged_attention(*args)
+    for _ in range(20):
+        assert torch.equal(ops.paged_attention(*args, work=work), want)
 
 
 def test_attention_nothing(ops):
