@@ -45,17 +45,17 @@ def _ptrs(name: str, *specs):
             raise ValueError(f"{name}: {what} must be contiguous {dtype} {list(shape)}, got {t.dtype} {list(t.shape)} "
                              f"strides {list(t.stride())}")
         d = t.get_device()
-        if idx is None:
+        if d != idx:
+            if idx is not None or d < 0:
+                raise ValueError(f"{name}: {what} is on {t.device}: every tensor must be on one GPU")
             idx = d
-        if d != idx or d < 0:
-            raise ValueError(f"{name}: {what} is on {t.device}: every tensor must be on one GPU")
         out.append(t.data_ptr())
     return idx, out
 
 
 def _launch(idx: int, name: str, fn, *args):
     """The C call on the current stream of the tensors' GPU, whatever the current device is."""
-    if idx == torch.cuda.current_device():
+    if idx == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):
@@ -67,7 +67,8 @@ def _launch(idx: int, name: str, fn, *args):
     ops._check(rc, name)
 
 
-def _aligned(name: str, **ptrs):
+def _misaligned(name: str, **ptrs):
+    """Says which: the callers look at all addresses at once first."""
     for what, p in ptrs.items():
         if p % 16:
             raise ValueError(f"{name}: {what} must start at a multiple of 16 bytes")
@@ -100,11 +101,10 @@ def page_plan(new_lens: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
     if its tokens fit (64 * W of them, and ``n_tokens`` rows in all) and the free pages reach for the pages of every
     request up to it; what it would have taken stays reserved for it ahead of later ones.  Nothing that is committed
     changes: planning again gives the same plan, and ``page_commit`` makes it so."""
-    if table.dim() != 2 or not 0 < table.shape[0] <= MAX_ROWS or table.shape[1] < 1 or free.dim() != 1 \
-            or free.numel() < 1:
-        raise ValueError(f"page_plan: table [B <= {MAX_ROWS}, W], free [pages], got {list(table.shape)} {list(free.shape)}")
-    B, W = table.shape
+    B, W = table.shape if table.dim() == 2 else (0, 0)
     pages = free.numel()
+    if not 0 < B <= MAX_ROWS or W < 1 or free.dim() != 1 or pages < 1:
+        raise ValueError(f"page_plan: table [B <= {MAX_ROWS}, W], free [pages], got {list(table.shape)} {list(free.shape)}")
     if n_tokens < 0 or max(pages, W) * PAGE > 2**31 - 1:
         raise ValueError(f"page_plan: n_tokens {n_tokens}, {pages} pages, {W} a request: slots are 32-bit")
     idx, p = _ptrs("page_plan", ("new_lens", new_lens, _I32, (B,)), ("lengths", lengths, _I32, (B,)),
@@ -218,8 +218,8 @@ def paged_qk_norm_rope_kv(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: t
     pages, specs = _cache_specs(cache, name, n_q_heads, n_kv_heads, head_dim)
     width = (n_q_heads + 2 * n_kv_heads) * head_dim
     N = positions.shape[0] if positions.dim() == 1 else -1
-    if qkv.dtype is not _BF16 or qkv.shape != (N, width) or (N > 0 and qkv.stride(1) != 1) \
-            or (N > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < width)):
+    ld, one = qkv.stride() if qkv.dim() == 2 else (0, 0)
+    if qkv.dtype is not _BF16 or qkv.shape != (N, width) or (N > 0 and one != 1) or (N > 1 and (ld % 8 or ld < width)):
         raise ValueError(f"{name}: qkv must be bf16 [{N}, {width}] with unit column stride and a row stride that is a "
                          f"multiple of 8, got {qkv.dtype} {list(qkv.shape)} strides {list(qkv.stride())}")
     idx, p = _ptrs(name, ("q_norm_w", q_norm_w, _BF16, (head_dim,)), ("k_norm_w", k_norm_w, _BF16, (head_dim,)),
@@ -227,9 +227,11 @@ def paged_qk_norm_rope_kv(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: t
                    ("turns", turns, _I64, (head_dim // 2,)), ("q_out", q_out, _BF16, (N, n_q_heads, head_dim)), *specs)
     if qkv.get_device() != idx:
         raise ValueError(f"{name}: qkv is on {qkv.device}: every tensor must be on one GPU")
-    _aligned(name, qkv=qkv.data_ptr(), q_norm_w=p[0], k_norm_w=p[1], q_out=p[5], k=p[6], v=p[7])
-    _launch(idx, name, ops.lib().mivgpu_paged_qk_norm_rope_kv, qkv.data_ptr(), qkv.stride(0) if N > 1 else width, *p, N,
-            n_q_heads, n_kv_heads, head_dim, pages, eps)
+    x = qkv.data_ptr()
+    if (x | p[0] | p[1] | p[5] | p[6] | p[7]) & 15:
+        _misaligned(name, qkv=x, q_norm_w=p[0], k_norm_w=p[1], q_out=p[5], k=p[6], v=p[7])
+    _launch(idx, name, ops.lib().mivgpu_paged_qk_norm_rope_kv, x, ld if N > 1 else width, *p, N, n_q_heads, n_kv_heads,
+            head_dim, pages, eps)
     return q_out
 
 
@@ -267,11 +269,11 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, table: torch.Tensor, cu_q: 
     if q.dim() != 3 or not 0 < scale < math.inf:
         raise ValueError(f"{name}: q must be [N, {n_q_heads}, {head_dim}], got {list(q.shape)}, and scale positive, got {scale}")
     N = q.shape[0]
-    if table.dim() != 2 or not 0 < table.shape[0] <= MAX_ROWS or table.shape[1] < 1 or table.shape[1] * PAGE > 2**31 - 1:
+    B, W = table.shape if table.dim() == 2 else (0, 0)
+    if not 0 < B <= MAX_ROWS or not 0 < W <= (2**31 - 1) // PAGE:
         raise ValueError(f"{name}: table must be [B <= {MAX_ROWS}, W], got {list(table.shape)}")
     if max_new is not None and not 0 <= max_new < 2**31:
         raise ValueError(f"{name}: max_new {max_new}")
-    B, W = table.shape
     if out is None:
         out = torch.zeros(N, n_q_heads * head_dim, dtype=_BF16, device=q.device)
     idx, p = _ptrs(name, ("q", q, _BF16, (N, n_q_heads, head_dim)), *specs, ("table", table, _I32, (B, W)),
@@ -281,7 +283,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, table: torch.Tensor, cu_q: 
         work = paged_attention_workspace(N, B, n_q_heads, n_kv_heads, head_dim, q.device)
     if work.dtype is not _F32 or work.dim() != 1 or not work.is_contiguous() or work.get_device() != idx:
         raise ValueError(f"{name}: work must be from paged_attention_workspace on {q.device}")
-    _aligned(name, q=p[0], k=p[1], v=p[2], out=p[8], work=work.data_ptr())
-    _launch(idx, name, ops.lib().mivgpu_paged_attention, *p, work.data_ptr(), work.numel(), N, B, W, n_q_heads, n_kv_heads,
+    room = work.data_ptr()
+    if (p[0] | p[1] | p[2] | p[8] | room) & 15:
+        _misaligned(name, q=p[0], k=p[1], v=p[2], out=p[8], work=room)
+    _launch(idx, name, ops.lib().mivgpu_paged_attention, *p, room, work.numel(), N, B, W, n_q_heads, n_kv_heads,
             head_dim, pages, -1 if max_new is None else max_new, scale)
     return out
