@@ -13,9 +13,12 @@
 // value by a scan over the lanes.  All waves make the same searches, so none waits for another.  Weights and sums are
 // 64-bit and in one fixed order: the same inputs give the same token.
 //
-// Bound: the LDS atomics of the count and the row's way into one CU, twice.  A workgroup of 1024 threads takes a row, so
-// up to 256 rows take the time of one.  Measured and left out (152k tokens, 1 row): the row kept in registers, 37 us
-// against 30 -- the loops unrolled for it run from cold instruction lines.
+// Bound: the LDS atomics of the count (14 of 29 us; 64 lanes on random banks, 14 cycles an instruction) and a chain of
+// latencies.  A workgroup of 1024 threads takes a row, so up to 256 rows take little more than one: 29 us for 1 row of
+// 152k tokens, 35 for 32 of mixed settings, 40 for 256.  Measured and left out: the row kept in registers (1 row 37 us
+// against 30) -- the loops unrolled for it run from cold instruction lines; few rows counted by eight workgroups each,
+// whose counts the last to arrive adds up (1 row 29.4 us against 29.5, 32 rows 37 against 35) -- leaving the counts,
+// arriving and reading them takes what the shorter count saves.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -232,13 +235,13 @@ sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, int turns,
   const double p = top_p != nullptr ? (double)top_p[b] : 1.0;
   const double mp = min_p != nullptr ? (double)min_p[b] : 0.0;
   const double u = uniform[b] < 0.f ? 0.0 : (double)uniform[b];
-  const double rT = (double)T;
+  const double rT = 1.0 / (double)T;    // one division a row: off by 2^-53 of the exponent
   int first = 0, ncarry = 0;
   float vmax = 0.f;
   // exp((value - max) / T); the largest value's is 1 whatever T and the value are
   auto weight = [&](int bin) {
     if (bin == first) return 1.0;
-    return isfinite(vmax) ? exp(((double)value_of(bin) - (double)vmax) / rT) : 0.0;
+    return isfinite(vmax) ? exp(((double)value_of(bin) - (double)vmax) * rT) : 0.0;
   };
   auto count_of = [&](int bin) {
     int c = (int)((hist[bin >> 1] >> (16 * (bin & 1))) & 0xffffu);

@@ -7,13 +7,15 @@ import torch
 from k8s_vgpu_scheduler_amd import ops
 from k8s_vgpu_scheduler_amd.ops.paged import _BF16, _F32, _I32, _I64, _launch, _ptrs
 
-MAX_VOCAB = 128 * 32768      # csrc/ops/sample.hip CARRIES * CHUNK
+MAX_VOCAB = 128 * 32768      # csrc/ops/sample.hip CARRIES * CARRY
 
 
 def sample_workspace(rows: int, vocab: int, device="cuda") -> torch.Tensor:
-    """Workspace of ``sample`` for up to ``rows`` rows of ``vocab`` logits.  Every call leaves it ready for the next;
-    calls that may run at once need one each."""
-    return torch.zeros(0, dtype=torch.int64, device=device)
+    """Workspace of ``sample`` for up to ``rows`` rows of ``vocab`` logits.  Empty: a row is counted and searched within
+    one workgroup."""
+    if rows < 1 or not 0 < vocab <= MAX_VOCAB:
+        raise ValueError(f"sample_workspace: {rows} rows of {vocab} logits (at most {MAX_VOCAB})")
+    return torch.empty(0, dtype=_I64, device=device)
 
 
 def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None,
@@ -44,5 +46,7 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tenso
                    ("tokens", tokens, _I64, (B,)), ("probs", probs, _F32, (B,)))
     if logits.get_device() != idx:
         raise ValueError(f"sample: logits are on {logits.device}: every tensor must be on one GPU")
+    if work is not None and (work.dtype is not _I64 or work.get_device() != idx):
+        raise ValueError(f"sample: work must be from sample_workspace on {logits.device}")
     _launch(idx, "sample", ops.lib().mivgpu_sample, logits.data_ptr(), logits.stride(0) if B > 1 else V, V, B, *p)
     return tokens, probs

@@ -151,6 +151,12 @@ def test_sample_refuses(bad):
         ops.sample(**sample_args(**bad))
 
 
+@pytest.mark.parametrize("args", [(0, 10), (1, 0), (1, 128 * 32768 + 1)])
+def test_sample_workspace_refuses(args):
+    with pytest.raises(ValueError, match="sample_workspace"):
+        ops.sample_workspace(*args, device="cpu")
+
+
 def test_oracle_plan_by_hand():
     """Two requests, one page short: the second is refused, the third needs none."""
     table = np.full((3, 4), -1)

@@ -203,6 +203,13 @@ def test_frequencies(ops):
     assert torch.all((got - want).abs() <= 1.0)
 
 
+def test_workspace_of_another_kind_is_refused(ops):
+    x = logits_of(1, 100, 0)
+    for work in (torch.zeros(0, device="cuda"), torch.zeros(0, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="sample"):
+            ops.sample(x, torch.zeros(1, device="cuda"), work=work)
+
+
 def test_greedy_is_decode_tail(ops):
     x = logits_of(8, 4096, 9)
     x[3, 1000] = math.nan
