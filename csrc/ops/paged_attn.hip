@@ -357,6 +357,7 @@ __device__ __forceinline__ void short_part(const Call& c, const Work& k, int upt
         pf[h][j] = (__bf16)e;
       }
     if (live < PAGE) {                            // slots never written may hold any code, NaN too
+      if (cur.bad) cur.vs = 1.f;                  // page 0's, which may never have been written either
       const uint32_t m0 = live_bytes(16 * a, live), m1 = live_bytes(16 * a + 4, live), m2 = live_bytes(16 * a + 8, live),
                      m3 = live_bytes(16 * a + 12, live);
 #pragma unroll
@@ -576,6 +577,7 @@ __device__ __forceinline__ void long_part(const Call& c, const Work& k, unsigned
       const int dim = t / (PAGE / 16), qk = t % (PAGE / 16), live = bad[z] ? 0 : L - p * PAGE;
       uint4& v = vr[z];
       if (live < PAGE) {                               // slots never written may hold any code, NaN too
+        if (bad[z]) vs[z] = 1.f;                       // page 0's, which may never have been written either
         v.x &= live_bytes(16 * qk, live);
         v.y &= live_bytes(16 * qk + 4, live);
         v.z &= live_bytes(16 * qk + 8, live);

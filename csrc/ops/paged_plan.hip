@@ -100,7 +100,7 @@ page_plan_kernel(const int* __restrict__ new_lens, const int* __restrict__ lengt
 
 // Takes the plan's pages out of the ring, sets the lengths and puts the pages of finished requests back, in the
 // order of the requests.  Pages taken follow from the lengths before and after, so committing a plan again takes
-// none.  One workgroup: a few KB.
+// none (but for a request that finished with it, whose length is then 0).  One workgroup: a few KB.
 __global__ void __launch_bounds__(NT)
 page_commit_kernel(const int* __restrict__ kv_lens, const int* __restrict__ taken, const uint8_t* __restrict__ finished,
                    int* __restrict__ lengths, const int* __restrict__ table, int* __restrict__ ring_pages,

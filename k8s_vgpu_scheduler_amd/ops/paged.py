@@ -129,7 +129,8 @@ def page_plan(new_lens: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
 def page_commit(plan: PagePlan, lengths: torch.Tensor, table: torch.Tensor, free: torch.Tensor, ring: torch.Tensor,
                 finished: torch.Tensor | None = None):
     """The plan's step is done: ``lengths`` of admitted requests become its ``kv_lens`` and their pages leave the
-    ring.  ``finished`` (bool [B]): requests whose pages go back to the ring's end, in order; their length becomes 0."""
+    ring.  ``finished`` (bool [B]): requests whose pages go back to the ring's end, in order; their length becomes 0.  A plan
+    is committed once."""
     if table.dim() != 2 or not 0 < table.shape[0] <= MAX_ROWS or table.shape[1] < 1 or free.dim() != 1 \
             or free.numel() < 1 or max(free.numel(), table.shape[1]) * PAGE > 2**31 - 1:
         raise ValueError(f"page_commit: table [B <= {MAX_ROWS}, W], free [pages], got {list(table.shape)} {list(free.shape)}")
@@ -198,8 +199,8 @@ def _cache_specs(cache: PagedKV, name: str, n_q_heads: int, n_kv_heads: int, hea
 def rope_turns(theta: float, head_dim: int, device="cuda") -> torch.Tensor:
     """The rotation's table: 2^64 * theta^(-2i/D) / 2pi for i < D/2, rounded, modulo 2^64 (int64 bits).  A
     position's angle in turns is the fraction position * turns / 2^64, exact to 2^-65 of the position."""
-    if head_dim not in (64, 128) or not theta > 0:
-        raise ValueError(f"rope_turns: theta {theta}, head_dim {head_dim} (64 or 128)")
+    if head_dim not in (64, 128) or not 1 <= theta < math.inf:
+        raise ValueError(f"rope_turns: theta {theta} (at least 1), head_dim {head_dim} (64 or 128)")
     vals = [round(theta ** (-2.0 * i / head_dim) / (2 * math.pi) * 2**64) % 2**64 for i in range(head_dim // 2)]
     return torch.tensor([v - 2**64 if v >= 2**63 else v for v in vals], dtype=torch.int64, device=device)
 

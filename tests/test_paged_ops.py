@@ -51,7 +51,7 @@ def test_rope_turns(d, theta):
     assert np.all(np.abs(got - want) <= want * 2.0 ** -48 + 2.0 ** -65)
 
 
-@pytest.mark.parametrize("theta,d", [(0.0, 128), (-1.0, 128), (1e6, 96), (math.nan, 128)])
+@pytest.mark.parametrize("theta,d", [(0.0, 128), (-1.0, 128), (1e6, 96), (math.nan, 128), (math.inf, 128), (1e-300, 128)])
 def test_rope_turns_refuses(theta, d):
     with pytest.raises(ValueError):
         ops.rope_turns(theta, d, device="cpu")

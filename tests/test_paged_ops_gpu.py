@@ -422,6 +422,22 @@ def test_attention_bad_pages(ops, new):
     assert (out[2 * new:3 * new] == 0).all()
 
 
+@pytest.mark.parametrize("new", [1, 50])
+def test_attention_bad_pages_beside_an_unwritten_first_page(ops, new):
+    """The cache's first page, never written: scales and codes of any bits.  Masked pages take nothing from it."""
+    q, cache, table, cu, kv = attention_case(ops, [200, 300, 20], [new] * 3, 4, 2, 128)
+    first = lambda t, v: torch.cat([torch.full_like(t[:1].view(torch.uint8), v), t.view(torch.uint8)]).view(t.dtype)  # noqa: E731
+    cache = ops.PagedKV(*(first(t, 0xff) for t in cache))      # NaN codes and NaN scales
+    table = table + 1
+    table[0, 1], table[1, 0], table[1, 3] = -1, cache.k.shape[0], 2**31 - 1
+    table[2, :] = -5
+    out = ops.paged_attention(q.cuda(), cache, dev(table), dev(cu), dev(kv), 4, 2, 128, 0.1)
+    assert out[:3 * new].isfinite().all() and (out[2 * new:3 * new] == 0).all()
+    for t in cache:
+        t[0].view(torch.uint8).zero_()
+    assert torch.equal(out, ops.paged_attention(q.cuda(), cache, dev(table), dev(cu), dev(kv), 4, 2, 128, 0.1))
+
+
 def test_attention_shared_pages(ops):
     """Two requests with the same prefix read the same pages."""
     q, cache, table, cu, kv = attention_case(ops, [128, 128], [1, 1], 4, 2, 128)
