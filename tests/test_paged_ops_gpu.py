@@ -404,6 +404,18 @@ def test_attention(ops, case):
     assert a.shape == b.shape
 
 
+@pytest.mark.parametrize("rows,long,seed", [(65, 0, 0), (130, 150, 1), (200, 0, 2), (1024, 100, 3)])
+def test_attention_many_requests(ops, rows, long, seed):
+    """More requests than a wave has lanes, some without tokens, with and without a chunk among them."""
+    r = np.random.RandomState(seed)
+    old, new = r.randint(0, 150, rows), r.randint(0, 3, rows)
+    old[r.randint(rows)] = 900
+    if long:
+        new[r.randint(rows)] = long
+    q, cache, table, cu, kv = attention_case(ops, old, new, 4, 2, 64, seed)
+    check_attention(ops, q, cache, table, cu, kv, 4, 2, 64)
+
+
 def test_attention_rows_that_see_nothing(ops):
     """A request that was not admitted (no keys), and one with fewer keys than rows: zeros where no key is seen."""
     q, cache, table, cu, kv = attention_case(ops, [10, 0, 20], [3, 5, 2], 4, 2, 128)
