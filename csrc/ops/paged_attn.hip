@@ -498,10 +498,11 @@ __device__ __forceinline__ void short_part(const Call& c, const Work& k, int upt
 // of a read cover all banks.
 // The output and sum are rescaled only where a row's maximum grew by more than 8 (in log2): the p stay below 2^8,
 // which neither bf16 nor the sums mind.
-// Measured on an 8192-token prompt, 32 / 8 heads: 515 us, 1067 TFLOP/s; with the stores before the barrier instead of
-// between the pages 525, a barrier a page 568, the buffers picked at run time 551.  The matrix units are busy less than
-// half of the time, the softmax of a SIMD's two waves and the stores take the rest: without the stores and loads it
-// would be 396.  Left out: the two waves of a SIMD half a page apart, one's matrix instructions beside the other's
+// Measured on an 8192-token prompt, 32 / 8 heads: 514 us, 1070 TFLOP/s; with the stores before the barrier instead of
+// between the pages 525, a barrier a page 568, the buffers picked at run time 551.  The matrix units are busy half
+// of the time and the vector units the other half, at a clock of 1.9 to 2.1 GHz of the card's 2.4: hiding more latency
+// gains nothing (operands read three steps ahead 511; the next page's scores beside this one's exponentials in a wave
+// 528), less work does (without the stores and loads it would be 396).  Left out: the two waves of a SIMD half a page apart, one's matrix instructions beside the other's
 // exponentials, two barriers a page (653; 614 without the offset); four waves of 64 rows, which halve the LDS reads,
 // the next page's scores beside this one's exponentials (792).
 template <int D>
@@ -558,6 +559,8 @@ __device__ __forceinline__ void long_part(const Call& c, const Work& k, unsigned
       const size_t x = (size_t)(ids < 0 || ids >= pages ? 0 : ids) * Hkv + hk;
       kss = kscale[x];
       vss = vscale[x];
+      // arrived: a wait here, every 64 pages, not behind the branch, where it would be for the codes on their way too
+      asm volatile("" : "+v"(ids), "+v"(kss), "+v"(vss));
     }
     const int id = __builtin_amdgcn_readlane(ids, at);
     ks[z] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), at));

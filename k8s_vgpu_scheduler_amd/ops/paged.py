@@ -111,8 +111,8 @@ def page_plan(new_lens: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
                    ("table", table, _I32, (B, W)), ("free", free, _I32, (pages,)), ("ring", ring, _I32, (2,)))
     sizes = (B + 1, B, B, n_tokens, n_tokens)
     if out is None:
-        buf = torch.empty(sum(sizes), dtype=_I32, device=table.device)     # one allocation
-        out = PagePlan(*torch.split_with_sizes(buf, sizes))
+        buf = free.new_empty(sum(sizes))                                   # one allocation
+        out = PagePlan(*torch.unsafe_split_with_sizes(buf, sizes))
         at = buf.data_ptr()
         for n in sizes:
             p.append(at)

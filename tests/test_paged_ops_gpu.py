@@ -194,6 +194,7 @@ APPENDS = {
     "one head each": ([1], [5], 1, 1, 64, 0, 0),
     "many heads": ([1, 2], [5, 1], 40, 8, 128, 0, 0),
     "long batch": ([0, 70], [1500, 3], 4, 2, 128, 0, 5),
+    "longer batch": ([0, 30, 64], [4200, 900, 1], 2, 1, 64, 0, 2),
 }
 
 
