@@ -499,18 +499,19 @@ __device__ __forceinline__ void short_part(const Call& c, const Work& k, int upt
 // The output and sum are rescaled only where a row's maximum grew by more than 8 (in log2): the p stay below 2^8,
 // which neither bf16 nor the sums mind.
 // Measured on an 8192-token prompt, 32 / 8 heads: 514 us, 1070 TFLOP/s; with the stores before the barrier instead of
-// between the pages 525, a barrier a page 568, the buffers picked at run time 551.  The matrix units are busy half
-// of the time and the vector units the other half, at a clock of 1.9 to 2.1 GHz of the card's 2.4: hiding more latency
+// between the pages 525, a barrier a page 568, the buffers picked at run time 551.  The matrix units are busy half of
+// the time and the vector units the other half, at a clock of 1.9 to 2.1 GHz of the card's 2.4: hiding more latency
 // gains nothing (operands read three steps ahead 511; the next page's scores beside this one's exponentials in a wave
-// 528), less work does (without the stores and loads it would be 396).  Left out: the two waves of a SIMD half a page apart, one's matrix instructions beside the other's
-// exponentials, two barriers a page (653; 614 without the offset); four waves of 64 rows, which halve the LDS reads,
-// the next page's scores beside this one's exponentials (792).
+// 528), less work does (without the stores and loads it would be 396).  Left out: the two waves of a SIMD half a page
+// apart, one's matrix instructions beside the other's exponentials, two barriers a page (653; 614 without the offset);
+// four waves of 64 rows, which halve the LDS reads, the next page's scores beside this one's exponentials (792).
 template <int D>
 __device__ __forceinline__ int k_at(int row, int ch) { return row * D + ((ch ^ (row & (D / 8 - 1))) << 3); }
 __device__ __forceinline__ int v_at(int dim, int ch) { return dim * PAGE + ((ch ^ ((dim >> 1) & 7)) << 3); }
 
 template <int D>
-__device__ __forceinline__ void long_part(const Call& c, const Work& k, unsigned block, bf16_t (&s_k)[4][PAGE * D], bf16_t (&s_v)[4][PAGE * D]) {
+__device__ __forceinline__ void long_part(const Call& c, const Work& k, unsigned block, bf16_t (&s_k)[4][PAGE * D],
+                                          bf16_t (&s_v)[4][PAGE * D]) {
   MIVGPU_PATTN_ARGS;
   constexpr int KS = D / 16, DC = D / 32;              // k-steps of the scores, 32-wide blocks of the output
   constexpr int CHUNKS = PAGE * D / 16;                // 16-byte chunks of codes in a page, each of K and V
