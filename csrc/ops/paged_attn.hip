@@ -6,7 +6,7 @@
 // in one pass over the pages with the running maximum m and sum (fp32).
 //
 // The rows of one kv head's G query heads are flattened (row = token * G + head) and cut into tiles: of 16 rows where
-// a request brings at most SHORT_ROWS of them (decode, a few tokens), of 256 in the others (chunks, prompts).  Both
+// a request brings few of them (short_rows: decode, a few tokens), of 256 in the others (chunks, prompts).  Both
 // kinds of workgroups are in one launch, so that the short ones' waits for memory lie beside the long ones' products (a
 // chunk of 855 tokens beside seven decoding requests: 80 us; in a launch each 90).
 // A tile's pages are split over as many workgroups as keep the chip evenly busy: every workgroup scans the requests'
@@ -41,10 +41,18 @@ constexpr int WAVES = 8, NT = 64 * WAVES, TILE = 16;
 constexpr int MIN_CHUNK = WAVES;         // pages of a part: at least one for each wave
 constexpr int MAX_PARTS = 256;           // of a tile: their (m, l) take 32 KB of LDS
 constexpr int JOIN = 64;                 // head dimensions that the waves join at once
-constexpr int SHORT_ROWS = 64;
 // long requests
 constexpr int LNT = 512, LWAVES = 8, LTILE = 32 * LWAVES;
 constexpr int LMIN_CHUNK = 8;
+
+// The most rows of a request that go in short tiles.  A short tile is soon done but reads its pages for 16 rows, a long
+// one takes 2 to 3 times as long for up to 256; calls of few rows have CUs over for short ones.  32 / 8 heads, 4096 keys
+// before the new ones, us short / long: 1 request of 64 rows 13 / 26, of 256 27 / 50; 4 of 64 28 / 29, of 128 31 / 35;
+// 16 of 64 56 / 87, of 128 109 / 87; 64 of 32 134 / 175, of 64 228 / 178.
+constexpr int FEW_ROWS = 512, MANY_ROWS = 4096;
+constexpr int short_rows(long long rows) {
+  return rows <= FEW_ROWS ? FEW_ROWS : rows < MANY_ROWS ? 64 : 32;
+}
 
 // A call aims at as many workgroups as are resident (two of the short ones with D = 64 a CU, otherwise one), over all kv
 // heads, and with that bounds the slots of the workspace: with t parts aimed at a kv head a split tile of np pages gets at
@@ -188,7 +196,7 @@ struct Call {
   const float *__restrict__ kscale, *__restrict__ vscale;
   const int *__restrict__ table, *__restrict__ cu, *__restrict__ kv_lens;
   bf16_t* __restrict__ out;
-  int N, B, W, Hq, Hkv, pages;
+  int N, B, W, Hq, Hkv, pages, upto;     // upto: the most rows of a request that short tiles take
   float scale_log2;
 };
 // Of one kind: its workspace, the parts it aims at for each kv head, and its workgroups
@@ -218,7 +226,7 @@ struct ShortLds {
   __attribute__((aligned(16))) char raw[O_BYTES > JOIN_BYTES ? O_BYTES : JOIN_BYTES];
 };
 
-// upto: the most rows of a request that the short tiles take
+// upto: as in Call, or all
 template <int D>
 __device__ __forceinline__ void short_part(const Call& c, const Work& k, int upto, unsigned block, ShortLds<D>& lds) {
   MIVGPU_PATTN_ARGS;
@@ -520,7 +528,7 @@ __device__ __forceinline__ void long_part(const Call& c, const Work& k, unsigned
   // kv head = workgroup mod Hkv: with 8 of them each XCD's L2 serves one head's pages
   const int G = Hq / Hkv, hk = block % Hkv;
   const Share sh =
-      find_share<LTILE, LMIN_CHUNK>(cu, kv_lens, N, B, W, G, target, SHORT_ROWS, INT_MAX, block / Hkv, Hkv, k.grid);
+      find_share<LTILE, LMIN_CHUNK>(cu, kv_lens, N, B, W, G, target, c.upto, INT_MAX, block / Hkv, Hkv, k.grid);
   if (sh.ns == 0) return;
   const int b = sh.b, ns = sh.ns, tile0 = sh.tile * LTILE, row0 = tile0 + 32 * w;
   const int tok0 = min(max(cu[b], 0), N), n = min(cu[b + 1], N) - tok0, rows = n * G;
@@ -787,10 +795,10 @@ __global__ void __launch_bounds__(NT, 2) attn_both_kernel(const Call c, const Wo
   if (blockIdx.x < longs.grid) {
     long_part<D>(c, longs, blockIdx.x, s_k, s_v);
   } else if constexpr (sizeof(ShortLds<D>) <= sizeof(s_k)) {
-    short_part<D>(c, shorts, SHORT_ROWS, blockIdx.x - longs.grid, *reinterpret_cast<ShortLds<D>*>(s_k));
+    short_part<D>(c, shorts, c.upto, blockIdx.x - longs.grid, *reinterpret_cast<ShortLds<D>*>(s_k));
   } else {
     __shared__ ShortLds<D> lds;
-    short_part<D>(c, shorts, SHORT_ROWS, blockIdx.x - longs.grid, lds);
+    short_part<D>(c, shorts, c.upto, blockIdx.x - longs.grid, lds);
   }
 }
 
@@ -805,7 +813,7 @@ static int all_cus() {
 }
 
 // The workspace, for any head size: counters (zero before the first call, left zero), then (m, l) and O of the short
-// and, where a call has more rows than SHORT_ROWS, of the long tiles' parts.
+// and, where a call has more than FEW_ROWS rows, of the long tiles' parts.
 constexpr long long ZEROED = SHORT_SLOTS + LONG_SLOTS * (LNT / 64);
 constexpr long long SHORT_FLOATS = (long long)SHORT_SLOTS * TILE * (2 + 128);
 constexpr long long LONG_FLOATS = (long long)LONG_SLOTS * LTILE * (2 + 128);
@@ -813,7 +821,7 @@ constexpr long long LONG_FLOATS = (long long)LONG_SLOTS * LTILE * (2 + 128);
 long long mivgpu_paged_attention_work(int N, int Hq, int Hkv, long long* zeroed) {
   if (N < 0 || Hq <= 0 || Hkv <= 0 || Hkv > MAX_HKV || Hq % Hkv) return -1;
   *zeroed = ZEROED;
-  return ZEROED + SHORT_FLOATS + ((long long)N * (Hq / Hkv) > SHORT_ROWS ? LONG_FLOATS : 0);
+  return ZEROED + SHORT_FLOATS + ((long long)N * (Hq / Hkv) > FEW_ROWS ? LONG_FLOATS : 0);
 }
 
 // max_new: the most new tokens of a request, or negative if not known
@@ -830,7 +838,8 @@ int mivgpu_paged_attention(const void* q, const void* kc, const void* vc, const 
   const long long rows = (long long)N * G, some = N < B ? N : B;
   // All rows through the short kernel where no request is long; then it also takes one that is longer than it was
   // said to be.
-  const bool longs = rows > SHORT_ROWS && (max_new < 0 || (long long)max_new * G > SHORT_ROWS);
+  const int upto = short_rows(rows);
+  const bool longs = rows > upto && (max_new < 0 || (long long)max_new * G > upto);
   if (work == nullptr || floats < ZEROED + SHORT_FLOATS + (longs ? LONG_FLOATS : 0)) return -2;
   // Parts: no more than the tiles there can be and `target` on top (each part but a tile's last is a whole chunk), nor
   // than all chunks of all tiles
@@ -842,13 +851,13 @@ int mivgpu_paged_attention(const void* q, const void* kc, const void* vc, const 
   const int resident = head_dim == 64 ? 2 * all_cus() : all_cus(), target = resident / Hkv > 1 ? resident / Hkv : 1;
   long long tiles = rows / TILE + some, each = (long long)N * ((G + TILE - 1) / TILE);
   if (tiles > each) tiles = each;          // a token adds no more tiles than its own rows fill
-  if (longs && tiles > some * (SHORT_ROWS / TILE)) tiles = some * (SHORT_ROWS / TILE);
-  const long long few = rows / (SHORT_ROWS + 1), ltiles = rows / LTILE + (few < some ? few : some);
+  if (longs && tiles > some * (upto / TILE)) tiles = some * (upto / TILE);
+  const long long few = rows / (upto + 1), ltiles = rows / LTILE + (few < some ? few : some);
   const long long parts = grid_of(tiles, target, MIN_CHUNK) * Hkv, lparts = grid_of(ltiles, ltarget, LMIN_CHUNK) * Hkv;
   if (tiles * W > INT_MAX || (longs && ltiles * W > INT_MAX) || parts > INT_MAX || lparts > INT_MAX) return -1;
   if (longs && parts + lparts > INT_MAX) return -1;
   const Call c = {(const bf16_t*)q, (const uint8_t*)kc, (const uint8_t*)vc, kscale, vscale, table, cu, kv_lens,
-                  (bf16_t*)out, N, B, W, Hq, Hkv, pages, scale * 1.4426950408889634f};
+                  (bf16_t*)out, N, B, W, Hq, Hkv, pages, upto, scale * 1.4426950408889634f};
   const Work shorts = {(int*)work, work + ZEROED, work + ZEROED + SHORT_SLOTS * TILE * 2, target, (unsigned)parts};
   float* lml = work + ZEROED + SHORT_FLOATS;
   const Work more = {(int*)work + SHORT_SLOTS, lml, lml + LONG_SLOTS * LTILE * 2, ltarget, (unsigned)lparts};

@@ -346,6 +346,10 @@ ATTNS = {
     "prompts": ([0, 0, 64], [65, 128, 191], 4, 4, 64),
     "chunk beside decode": ([500, 77, 0, 200], [130, 1, 40, 1], 8, 2, 128),
     "chunk beside decode, heads of 64": ([700, 77, 0, 200], [300, 1, 40, 1], 4, 4, 64),
+    "prompts, heads of 64": ([0, 0, 64], [65, 328, 391], 4, 4, 64),
+    "chunk beside a few, heads of 64": ([700, 77, 0, 200, 30], [600, 1, 40, 17, 16], 8, 4, 64),
+    "a few each of many": ([200] * 30, [33, 8, 9, 16, 64] * 6, 16, 2, 128),
+    "few rows": ([300, 10], [100, 27], 8, 2, 128),
     "rows without tokens": ([10, 50, 0], [0, 2, 0], 4, 2, 128),
     "ragged decode": ([3000, 1, 70, 900, 0, 511, 64, 2100], [1] * 8, 16, 2, 128),
     "long chunk": ([700], [600], 4, 1, 128),
@@ -425,7 +429,7 @@ def test_attention_rows_that_see_nothing(ops):
     assert (out[3:5] == 0).all() and (out[8:10] == 0).all() and (out[5:8] != 0).any()
 
 
-@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("new", [1, 50, 200])
 def test_attention_bad_pages(ops, new):
     """A page that the cache does not have counts as masked; a row left with none gives zeros."""
     q, cache, table, cu, kv = attention_case(ops, [200, 300, 20], [new] * 3, 4, 2, 128)
@@ -435,7 +439,7 @@ def test_attention_bad_pages(ops, new):
     assert (out[2 * new:3 * new] == 0).all()
 
 
-@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("new", [1, 50, 200])
 def test_attention_bad_pages_beside_an_unwritten_first_page(ops, new):
     """The cache's first page, never written: scales and codes of any bits.  Masked pages take nothing from it."""
     q, cache, table, cu, kv = attention_case(ops, [200, 300, 20], [new] * 3, 4, 2, 128)
@@ -458,7 +462,7 @@ def test_attention_shared_pages(ops):
     check_attention(ops, q, cache, table, cu, kv, 4, 2, 128)
 
 
-@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("new", [1, 40, 200])
 def test_attention_nan_key(ops, new):
     """A NaN key reaches exactly the rows that see it, in its head."""
     q, cache, table, cu, kv = attention_case(ops, [70, 70], [new, new], 4, 2, 128)
@@ -515,7 +519,7 @@ def test_attention_more_new_tokens_than_said(ops):
         check_attention(ops, q, cache, table, cu, kv, 8, 2, 128, max_new=said)
 
 
-@pytest.mark.parametrize("new", [3, 90])
+@pytest.mark.parametrize("new", [3, 90, 300])
 def test_attention_overlapping_requests_stay_in_bounds(ops, new):
     """Rows that several requests claim have no answer, but nothing outside them is touched and the next call is right."""
     q, cache, table, cu, kv = attention_case(ops, [2000] * 6, [new] * 6, 4, 2, 128)
