@@ -13,9 +13,10 @@
 // NaN through its score, and a query that does not see it cannot be reached through 0 * NaN in the product with V.
 //
 // Bound: HBM (the rows once in, q and the codes once out).  Two kinds of workgroups in one launch:
-//   * K/V: one for each kv head and run of up to `window` tokens.  It takes every segment (consecutive slots of one
-//     page) that starts in its run, whole: the page's scale needs all of the segment's values, which 256 threads hold
-//     in registers (64 tokens x D values of K and of V), so nothing is read twice.  A thread has 8 dimensions of 4 (D =
+//   * K/V: some for each kv head and window of 256 tokens, which the segments (consecutive slots of one page) that
+//     start there are dealt out to.  A segment is taken whole: the page's scale needs all of its values, which 256
+//     threads hold in registers (64 tokens x D values of K and of V), so nothing is read twice; one within 16 slots, a
+//     decoding request's token above all, is a single wave's, without a barrier.  A thread has 8 dimensions of 4 (D =
 //     128) or 2 neighbouring slots, so that its V codes are whole words of V's rows [D][64];
 //   * q: waves of one token each; a lane keeps its 8 sines and cosines for the heads that it walks through.
 // Sines and cosines are the hardware's, which take turns: off by 2^-22.9 at most over [-1/2, 1/2] (all multiples of
@@ -27,6 +28,9 @@ using namespace paged;
 namespace {
 
 constexpr int NT = 256;
+constexpr int GROUP = 16;                        // slots of a wave, aligned
+// Tokens whose segments are dealt out together, and the fewest workgroups for them
+constexpr int WINDOW = 256, EACH = 4, LIST = WINDOW / EACH;
 
 template <int D>
 struct Head {
@@ -90,75 +94,40 @@ __device__ __forceinline__ void store_slots(uint8_t* row, int first, uint32_t w,
   }
 }
 
+// One segment (consecutive slots of one page, from token i on) of one kv head: by the whole workgroup, or by one wave
+// where it lies in one group of the wave's 16 slots.
 template <int D>
-__global__ void __launch_bounds__(NT, 3)
-append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __restrict__ qw, const bf16_t* __restrict__ kw,
-              const int* __restrict__ positions, const int* __restrict__ slots,
-              const unsigned long long* __restrict__ turns, bf16_t* __restrict__ q_out, uint8_t* __restrict__ kc,
-              uint8_t* __restrict__ vc, float* __restrict__ kscale, float* __restrict__ vscale, int N, int Hq, int Hkv,
-              int pages, int window, unsigned share, int spread, float eps) {
-  constexpr int LANES = Head<D>::LANES, ROWS = Head<D>::ROWS, PASS = PAGE / ROWS, WROWS = 64 / LANES;
-  __shared__ float red[2][NT / 64];
-  const int t = threadIdx.x, lane = t & 63, l = t % LANES;
-  float w[8], c[8], s[8];
+struct Append {
+  const bf16_t* __restrict__ qkv;
+  long long ld;
+  const bf16_t* __restrict__ kw;
+  const int *__restrict__ positions, *__restrict__ slots;
+  const unsigned long long* __restrict__ turns;
+  uint8_t *__restrict__ kc, *__restrict__ vc;
+  float *__restrict__ kscale, *__restrict__ vscale;
+  int N, Hq, Hkv;
+  float eps;
 
-  // The two kinds take turns, so that the K/V workgroups' latencies lie beside the q workgroups' traffic (8192 tokens: 50
-  // us against 76 with the K/V ones first).  kv: K/V workgroups before this one; share: their part of all, times 2^32
-  const unsigned me = blockIdx.x;
-  const int kv = (int)__umulhi(me, share);
-  if ((int)__umulhi(me + 1, share) == kv) {      // ---- q: a wave has every spread-th group of WROWS heads of a token
-    const int x = ((int)me - kv) * (NT / 64) + (t >> 6), i = x / spread;
-    if (i >= N) return;
-    const bf16_t* row = qkv + (size_t)i * ld + 8 * l;
-    bf16_t* to = q_out + (size_t)i * Hq * D + 8 * l;
-    unpack8(*reinterpret_cast<const uint4*>(qw + 8 * l), w);
-    {
-      unsigned long long f[8];
-      fractions<D>(positions[i], turns, l, f);
-      angles(f, c, s);
-    }
-    constexpr int AHEAD = 4;                     // heads on their way
-    const int step = WROWS * spread;
-    for (int h0 = x % spread * WROWS + lane / LANES; h0 < Hq + WROWS; h0 += AHEAD * step) {   // whole waves
-      uint4 in[AHEAD];
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) in[j] = *reinterpret_cast<const uint4*>(row + (size_t)min(h0 + j * step, Hq - 1) * D);
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        float y[8];
-        unpack8(in[j], y);
-        norm_rope<D>(y, w, c, s, l, eps);
-        if (h0 + j * step < Hq)
-          *reinterpret_cast<uint4*>(to + (size_t)(h0 + j * step) * D) =
-              make_uint4(pack2bf(y[0], y[1]), pack2bf(y[2], y[3]), pack2bf(y[4], y[5]), pack2bf(y[6], y[7]));
-      }
-    }
-    return;
-  }
-
-  // ---- K/V of one kv head: the segments that start in tokens [i0, i0 + window)
-  const int hk = kv % Hkv, i0 = kv / Hkv * window;
-  const int slot0 = t / LANES * PASS;            // of the thread's PASS slots
-  const long long limit = (long long)pages * PAGE;
-  unsigned long long heads;                      // tokens of the run that start a segment
-  {
-    const int i = i0 + lane, slot = lane < window && i < N ? slots[i] : -1;
-    heads = __ballot(slot >= 0 && slot < limit && (slot % PAGE == 0 || i == 0 || slots[max(i - 1, 0)] != slot - 1));
-  }
-  for (; heads != 0; heads &= heads - 1) {
-    const int i = i0 + __ffsll((long long)heads) - 1, slot = slots[i], off = slot % PAGE;
+  template <bool WAVE>
+  __device__ __forceinline__ void segment(int i, int hk, float (*red)[NT / 64]) const {
+    constexpr int LANES = Head<D>::LANES, ROWS = Head<D>::ROWS, PASS = PAGE / ROWS;
+    static_assert(64 / LANES * PASS == GROUP, "a wave's slots");
+    const int t = threadIdx.x, lane = t & 63, l = t % LANES;
+    const int slot = slots[i], off = slot % PAGE;
     // its length: tokens whose slots go on in the page
     const bool more = lane + off < PAGE && i + lane < N && slots[min(i + lane, N - 1)] == slot + lane;
     const unsigned long long run = __ballot(more);
     const int cnt = run == ~0ull ? 64 : __ffsll((long long)~run) - 1, end = off + cnt;
     const size_t ph = (size_t)(slot / PAGE) * Hkv + hk;
     const float ko = off > 0 ? kscale[ph] : 0.f, vo = off > 0 ? vscale[ph] : 0.f;
+    const int wslot = WAVE ? off & ~(GROUP - 1) : (t & ~63) / LANES * PASS;  // the wave's slots: GROUP from here
+    const int slot0 = wslot + lane / LANES * PASS;                           // of the thread's PASS slots
 
+    float w[8], c[8], s[8];
     float kf[PASS][8], ka = 0.f, va = 0.f;
     uint4 vin[PASS];
     unsigned bads = 0;                           // of the thread's slots: not finite
-    const int wslot = (t & ~63) / LANES * PASS;  // the wave's slots: WROWS * PASS from here
-    const bool busy = wslot < end && wslot + WROWS * PASS > off;
+    const bool busy = WAVE || (wslot < end && wslot + GROUP > off);
     if (busy) {
       uint4 kin[PASS];
       int pos[PASS];
@@ -204,10 +173,13 @@ append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __rest
         va = fmaxf(va, __shfl_xor(va, o, 64));
       }
     }
-    if (lane == 0) red[0][t >> 6] = ka, red[1][t >> 6] = va;
-    __syncthreads();                             // and every thread has the old scales
-    ka = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    va = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+    if (!WAVE) {
+      if (lane == 0) red[0][t >> 6] = ka, red[1][t >> 6] = va;
+      __syncthreads();                           // and every thread has the old scales
+      ka = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+      va = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+    }
+    const int me = WAVE ? lane : t, all = WAVE ? 64 : NT;
     float ks = exp2i(scale_exp(ka)), vs = exp2i(scale_exp(va));
     float kr = 1.f, vr = 1.f;                    // what the older codes are multiplied by
     if (off > 0) {
@@ -216,18 +188,18 @@ append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __rest
       kr = ko / ks;
       vr = vo / vs;
     }
-    if (t == 0) kscale[ph] = ks, vscale[ph] = vs;
+    if (me == 0) kscale[ph] = ks, vscale[ph] = vs;
     const float ki = 1.f / ks, vi = 1.f / vs;    // powers of two: exact
     uint8_t* kp = kc + ph * PAGE * D;
     uint8_t* vp = vc + ph * PAGE * D;
     if (kr != 1.f) {
-      for (int x4 = t; x4 < off * (D / 4); x4 += NT) {
+      for (int x4 = me; x4 < off * (D / 4); x4 += all) {
         uint32_t* at = reinterpret_cast<uint32_t*>(kp) + x4;
         *at = rescale4(*at, kr);
       }
     }
     if (vr != 1.f) {
-      for (int x4 = t; x4 < D * (PAGE / 4); x4 += NT) {
+      for (int x4 = me; x4 < D * (PAGE / 4); x4 += all) {
         uint8_t* row = vp + (size_t)(x4 / (PAGE / 4)) * PAGE;
         const int first = x4 % (PAGE / 4) * 4;
         if (first < off) store_slots<4>(row, first, rescale4(*reinterpret_cast<uint32_t*>(row + first), vr), 0, off);
@@ -257,8 +229,94 @@ append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __rest
         store_slots<PASS>(vp + (size_t)(8 * l + e) * PAGE, slot0, to_codes(code(0), code(1), code(PASS - 2), code(PASS - 1)), off, end);
       }
     }
-    __syncthreads();                             // red is free for the next segment
+    if (!WAVE) __syncthreads();                  // red is free for the next segment
   }
+};
+
+template <int D>
+__global__ void __launch_bounds__(NT, 3)
+append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __restrict__ qw, const bf16_t* __restrict__ kw,
+              const int* __restrict__ positions, const int* __restrict__ slots,
+              const unsigned long long* __restrict__ turns, bf16_t* __restrict__ q_out, uint8_t* __restrict__ kc,
+              uint8_t* __restrict__ vc, float* __restrict__ kscale, float* __restrict__ vscale, int N, int Hq, int Hkv,
+              int pages, int each, unsigned share, int spread, float eps) {
+  constexpr int LANES = Head<D>::LANES, WROWS = 64 / LANES;
+  __shared__ float red[2][NT / 64];
+  __shared__ int sums[NT / 64], found[2][LIST];
+  const int t = threadIdx.x, lane = t & 63, l = t % LANES;
+
+  // The two kinds take turns, so that the K/V workgroups' latencies lie beside the q workgroups' traffic (8192 tokens: 50
+  // us against 76 with the K/V ones first).  kv: K/V workgroups before this one; share: their part of all, times 2^32
+  const unsigned me = blockIdx.x;
+  const int kv = (int)__umulhi(me, share);
+  if ((int)__umulhi(me + 1, share) == kv) {      // ---- q: a wave has every spread-th group of WROWS heads of a token
+    const int x = ((int)me - kv) * (NT / 64) + (t >> 6), i = x / spread;
+    if (i >= N) return;
+    const bf16_t* row = qkv + (size_t)i * ld + 8 * l;
+    bf16_t* to = q_out + (size_t)i * Hq * D + 8 * l;
+    float w[8], c[8], s[8];
+    unpack8(*reinterpret_cast<const uint4*>(qw + 8 * l), w);
+    {
+      unsigned long long f[8];
+      fractions<D>(positions[i], turns, l, f);
+      angles(f, c, s);
+    }
+    constexpr int AHEAD = 4;                     // heads on their way
+    const int step = WROWS * spread;
+    for (int h0 = x % spread * WROWS + lane / LANES; h0 < Hq + WROWS; h0 += AHEAD * step) {   // whole waves
+      uint4 in[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) in[j] = *reinterpret_cast<const uint4*>(row + (size_t)min(h0 + j * step, Hq - 1) * D);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        float y[8];
+        unpack8(in[j], y);
+        norm_rope<D>(y, w, c, s, l, eps);
+        if (h0 + j * step < Hq)
+          *reinterpret_cast<uint4*>(to + (size_t)(h0 + j * step) * D) =
+              make_uint4(pack2bf(y[0], y[1]), pack2bf(y[2], y[3]), pack2bf(y[4], y[5]), pack2bf(y[6], y[7]));
+      }
+    }
+    return;
+  }
+
+  // ---- K/V of one kv head: the window's segments, dealt out to its `each` workgroups, the short ones to their waves.
+  // Every workgroup goes through the window's slots: a few KB.
+  const int hk = kv % Hkv, mine = kv / Hkv % each, i0 = kv / Hkv / each * WINDOW, n = min(WINDOW, N - i0);
+  const long long limit = (long long)pages * PAGE;
+  const Append<D> to = {qkv, ld, kw, positions, slots, turns, kc, vc, kscale, vscale, N, Hq, Hkv, eps};
+  // 0: token i (slot `slot`, behind `before`) starts no segment; 1: one within a group of a wave's slots; 2: a longer one
+  auto ahead = [&](int slot) { return GROUP - (slot & (GROUP - 1)); };
+  auto kind = [&](int i, int slot, int before, int next) {
+    if (i >= N || slot < 0 || slot >= limit || (slot % PAGE != 0 && i > 0 && before == slot - 1)) return 0;
+    const int left = ahead(slot);
+    return slot % PAGE + left < PAGE && i + left < N && next == slot + left ? 2 : 1;
+  };
+  if (n <= each) {                               // a token each
+    const int i = i0 + mine;
+    if (i >= N) return;
+    const int slot = slots[i], k = kind(i, slot, slots[max(i - 1, 0)], slots[min(i + ahead(slot), N - 1)]);
+    if (k == 2) to.template segment<false>(i, hk, red);
+    if (k == 1 && t < 64) to.template segment<true>(i, hk, red);
+    return;
+  }
+  // A thread for each token.  Both kinds' numbers in one word
+  static_assert(WINDOW == NT, "a token a thread");
+  int k = 0;
+  {
+    const int i = min(i0 + t, N - 1), slot = slots[i], before = slots[max(i - 1, 0)];
+    if (t < n) k = kind(i, slot, before, slots[min(i + ahead(slot), N - 1)]);
+  }
+  const int one = k == 1 ? 1 : k == 2 ? 1 << 16 : 0;
+  int all;
+  const int at = block_scan<NT>(one, sums, &all) - one, no = k == 1 ? at & 0xffff : at >> 16;
+  if (k != 0 && no % each == mine) found[k - 1][no / each] = i0 + t;
+  __syncthreads();
+  const int shorts = all & 0xffff, longs = all >> 16;
+  for (int x = 0; x * each + mine < longs; ++x)
+    to.template segment<false>(__builtin_amdgcn_readfirstlane(found[1][x]), hk, red);
+  for (int x = t >> 6; x * each + mine < shorts; x += NT / 64)
+    to.template segment<true>(__builtin_amdgcn_readfirstlane(found[0][x]), hk, red);
 }
 
 }  // namespace
@@ -272,13 +330,18 @@ int mivgpu_paged_qk_norm_rope_kv(const void* qkv, long long ld, const void* qw, 
   if (N < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || pages <= 0 || (long long)pages * PAGE > INT_MAX) return -1;
   if (ld < (long long)(Hq + 2 * Hkv) * head_dim || ld % 8) return -1;
   if (N == 0) return 0;
-  // A decode step has a segment for each token: a workgroup for each.  In a longer batch (of at most 1024 requests, as
-  // everywhere here) ever more tokens lie inside segments: runs of 16 or 64 keep the workgroups that find nothing few.
-  const int window = N <= 1024 ? 1 : N < 4096 ? 16 : 64;
-  const long long nkv = (long long)((N + window - 1) / window) * Hkv;
-  // q: few tokens spread their heads over several waves; from 1024 tokens on there are waves enough
+  // Segments: up to one a token in a decode step, one for 64 in a prompt, and any mixture.  Few tokens have a workgroup
+  // each, more are dealt out to about 1024 (768 are resident): 1024 decoding requests 30 us, 8192 tokens of a prompt 39,
+  // 4000 beside 1000 decoding requests 57 (the same buffers again and again).  With a run of 1, 16 or 64 tokens a
+  // workgroup, its segments one by one, the first take 65, 80 and 284, the second 88, 47 and 39, the third 104, 84 and
+  // 300; with windows of 8192 tokens 32, 59 and 58.
+  const int windows = (N + WINDOW - 1) / WINDOW, resident = (1024 + windows * Hkv - 1) / (windows * Hkv);
+  const int most = resident > EACH ? resident : EACH, each = N < most ? N : most;
+  const long long nkv = (long long)windows * each * Hkv;
+  // q: from 1024 tokens on there are waves enough, fewer spread their heads over two (8 tokens 6.4 us against 6.8, 512 of
+  // a prompt 9.0 against 9.9; but 4096 25.8 against 24.5, and over four waves 29)
   const int groups = (Hq * head_dim / 8 + 63) / 64;
-  const int spread = N >= 1024 ? 1 : groups < 8 ? groups : 8;
+  const int spread = N >= 1024 || groups < 2 ? 1 : 2;
   const long long nq = ((long long)N * spread + NT / 64 - 1) / (NT / 64);
   if (nkv + nq > INT_MAX || (long long)N * spread > INT_MAX) return -1;
   const dim3 grid((unsigned)(nkv + nq));
@@ -287,7 +350,7 @@ int mivgpu_paged_qk_norm_rope_kv(const void* qkv, long long ld, const void* qw, 
 #define MIVGPU_APPEND(DD)                                                                                            \
   hipLaunchKernelGGL(append_kernel<DD>, grid, dim3(NT), 0, s, (const bf16_t*)qkv, ld, (const bf16_t*)qw,             \
                      (const bf16_t*)kw, positions, slots, (const unsigned long long*)turns, (bf16_t*)q_out,          \
-                     (uint8_t*)kc, (uint8_t*)vc, kscale, vscale, N, Hq, Hkv, pages, window, share, spread, eps)
+                     (uint8_t*)kc, (uint8_t*)vc, kscale, vscale, N, Hq, Hkv, pages, each, share, spread, eps)
   if (head_dim == 128) MIVGPU_APPEND(128);
   else if (head_dim == 64) MIVGPU_APPEND(64);
   else return -1;
