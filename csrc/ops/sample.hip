@@ -14,7 +14,7 @@
 // 64-bit and in one fixed order: the same inputs give the same token.
 //
 // Bound: the LDS atomics of the count (14 of 29 us; 64 lanes on random banks, 14 cycles an instruction) and a chain of
-// latencies.  A workgroup of 1024 threads takes a row, so up to 256 rows take little more than one: 29 us for 1 row of
+// latencies.  A workgroup of 1024 threads takes a row, so up to 256 rows take little more than one: 30 us for 1 row of
 // 152k tokens, 35 for 32 of mixed settings, 40 for 256.  Measured and left out: the row kept in registers (1 row 37 us
 // against 30) -- the loops unrolled for it run from cold instruction lines; few rows counted by eight workgroups each,
 // whose counts the last to arrive adds up (1 row 29.4 us against 29.5, 32 rows 37 against 35) -- leaving the counts,
