@@ -294,7 +294,7 @@ append_kernel(const bf16_t* __restrict__ qkv, long long ld, const bf16_t* __rest
   };
   if (n <= each) {                               // a token each
     const int i = i0 + mine;
-    if (i >= N) return;
+    if (mine >= n) return;                       // the next window's, or none
     const int slot = slots[i], k = kind(i, slot, slots[max(i - 1, 0)], slots[min(i + ahead(slot), N - 1)]);
     if (k == 2) to.template segment<false>(i, hk, red);
     if (k == 1 && t < 64) to.template segment<true>(i, hk, red);
@@ -336,7 +336,7 @@ int mivgpu_paged_qk_norm_rope_kv(const void* qkv, long long ld, const void* qw, 
   // workgroup, its segments one by one, the first take 65, 80 and 284, the second 88, 47 and 39, the third 104, 84 and
   // 300; with windows of 8192 tokens 32, 59 and 58.
   const int windows = (N + WINDOW - 1) / WINDOW, resident = (1024 + windows * Hkv - 1) / (windows * Hkv);
-  const int most = resident > EACH ? resident : EACH, each = N < most ? N : most;
+  const int most = resident < EACH ? EACH : resident > WINDOW ? WINDOW : resident, each = N < most ? N : most;
   const long long nkv = (long long)windows * each * Hkv;
   // q: from 1024 tokens on there are waves enough, fewer spread their heads over two (8 tokens 6.4 us against 6.8, 512 of
   // a prompt 9.0 against 9.9; but 4096 25.8 against 24.5, and over four waves 29)

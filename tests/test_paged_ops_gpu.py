@@ -196,6 +196,7 @@ APPENDS = {
     "long batch": ([0, 70], [1500, 3], 4, 2, 128, 0, 5),
     "prompts beside many": ([5, 63, 64, 100] * 80 + [0, 20], [1] * 320 + [700, 90], 2, 1, 64, 0, 3),
     "a few each of many": ([5, 63, 0, 50, 16] * 60, [3, 16, 40, 14, 17] * 60, 2, 2, 128, 0, 0),
+    "one kv head, more tokens than a window": ([18, 50, 62] * 150, [1] * 450, 2, 1, 64, 0, 1),
     "longer batch": ([0, 30, 64], [4200, 900, 1], 2, 1, 64, 0, 2),
 }
 
