@@ -313,6 +313,26 @@ def test_append_huge_values(ops):
     check_append(ops, [0], [5], 4, 2, 128, mend=mend)
 
 
+@pytest.mark.parametrize("hkv,d,seed", [(1, 64, 0), (1, 128, 1), (3, 64, 2), (8, 128, 3)])
+def test_append_in_one_call_or_many(ops, hkv, d, seed):
+    """Every bit is the same, however the requests are dealt out: prompts, chunks, a few tokens each and single ones."""
+    r = np.random.RandomState(seed)
+    new = r.choice([0, 1, 1, 2, 5, 16, 33, 70], 250)
+    new[r.randint(250)] = 1500
+    pos, slots, _, pages = layout(r.randint(0, 300, 250), new, seed)
+    hq, n, start = 2 * hkv, int(new.sum()), np.concatenate([[0], np.cumsum(new)])
+    qkv = torch.randn(n, (hq + 2 * hkv) * d, device="cuda").to(torch.bfloat16) * 2
+    w, turns = torch.ones(d, dtype=torch.bfloat16, device="cuda"), ops.rope_turns(THETA, d)
+    got = []
+    for cuts in ([0, 250], range(0, 251, 10)):
+        cache, q = filled_cache(ops, pages, hkv, d, seed), torch.zeros(n, hq, d, dtype=torch.bfloat16, device="cuda")
+        for a, b in zip(cuts, list(cuts)[1:]):
+            i, j = start[a], start[b]
+            ops.paged_qk_norm_rope_kv(qkv[i:j], w, w, dev(pos[i:j]), dev(slots[i:j]), turns, cache, q[i:j], hq, hkv, d, EPS)
+        got.append([t.view(torch.uint8) for t in (*cache, q)])
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
 def test_append_slots_outside_the_cache(ops):
     """Rows whose slot is negative or past the last page append nothing; q is written for all."""
     cache = filled_cache(ops, 3, 2, 128, 1)
