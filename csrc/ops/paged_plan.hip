@@ -74,12 +74,13 @@ page_plan_kernel(const int* __restrict__ new_lens, const int* __restrict__ lengt
   __syncthreads();
 
   const long long h = ((long long)head % num + num) % num;   // in bounds whatever the ring says
-  const int stride = gridDim.x * NT;
-  for (int i = blockIdx.x * NT + t; i < N; i += stride) {
-    const int b = upper_bound(s_end, B, i);
+  // (unsigned: one stride past N up to 2^31 - 1 does not wrap)
+  const unsigned stride = gridDim.x * NT, first = blockIdx.x * NT + t;
+  for (unsigned i = first; i < (unsigned)N; i += stride) {
+    const int b = upper_bound(s_end, B, (int)i);
     int pos = 0, slot = -1;
     if (b < B && s_len[b] >= 0) {
-      pos = s_len[b] + i - (b > 0 ? s_end[b - 1] : 0);
+      pos = s_len[b] + ((int)i - (b > 0 ? s_end[b - 1] : 0));
       const int j = pos / PAGE, have = (int)pages_of(s_len[b]);
       const int page = j < have ? table[(size_t)b * W + j] : ring_pages[(h + s_first[b] + j - have) % num];
       slot = page * PAGE + pos % PAGE;
@@ -88,11 +89,11 @@ page_plan_kernel(const int* __restrict__ new_lens, const int* __restrict__ lengt
     slots[i] = slot;
   }
   // new entries: they lie past the committed pages, which are all that the loop above reads
-  const int pages = (int)min(all, (long long)max(count, 0));
-  for (int k = blockIdx.x * NT + t; k < pages; k += stride) {
-    const int b = upper_bound(s_cum, B, k);
+  const unsigned pages = (unsigned)min(all, (long long)max(count, 0));
+  for (unsigned k = first; k < pages; k += stride) {
+    const int b = upper_bound(s_cum, B, (int)k);
     if (b < B && s_len[b] >= 0) {
-      const int j = (int)pages_of(s_len[b]) + k - s_first[b];
+      const int j = (int)pages_of(s_len[b]) + ((int)k - s_first[b]);
       table[(size_t)b * W + j] = ring_pages[(h + k) % num];
     }
   }
@@ -161,7 +162,7 @@ int mivgpu_page_plan(const int* new_lens, const int* lengths, int* table, const 
   if (B <= 0 || B > MAX_ROWS || W <= 0 || num <= 0 || N < 0 || (long long)num * PAGE > INT_MAX ||
       (long long)W * PAGE > INT_MAX)
     return -1;
-  const int grid = max(1, min((N + NT - 1) / NT, 1024));
+  const int grid = N > 1024 * NT ? 1024 : max(1, (N + NT - 1) / NT);
   hipLaunchKernelGGL(page_plan_kernel, dim3(grid), dim3(NT), 0, s, new_lens, lengths, table, ring_pages, ring, cu,
                      kv_lens, taken, positions, slots, B, W, num, N);
   return (int)hipGetLastError();

@@ -706,3 +706,13 @@ def test_two_streams(ops):
     torch.cuda.synchronize()
     for s, (att, tok) in zip(servers, want):
         assert torch.equal(s["att"][1], att) and torch.equal(s["tokens"], tok)
+
+
+def test_plan_of_as_many_rows_as_there_are_indices(ops):
+    """2^31 - 1 rows of which 75 hold a token: the walk over them ends at the last one."""
+    pool, n = ops.PagePool(40, 3, 6), 2**31 - 1
+    small, plan = pool.plan(dev([5, 70, 0]), 75), pool.plan(dev([5, 70, 0]), n)
+    assert plan.slots.shape == (n,) and plan.cu_q.tolist() == [0, 5, 75, 75] and plan.taken.tolist() == [1, 2, 0]
+    assert torch.equal(plan.slots[:75], small.slots) and torch.equal(plan.positions[:75], small.positions)
+    for t, v in ((plan.slots, -1), (plan.positions, 0)):
+        assert int(t[75:].amin()) == v and int(t[75:].amax()) == v
