@@ -18,6 +18,7 @@ captured by ``torch.cuda.CUDAGraph``.
 from __future__ import annotations
 
 import ctypes
+import decimal
 import math
 from typing import NamedTuple
 
@@ -196,13 +197,22 @@ def _cache_specs(cache: PagedKV, name: str, n_q_heads: int, n_kv_heads: int, hea
 
 
 # ----------------------------------------------------------------- append --
+_PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+
+
 def rope_turns(theta: float, head_dim: int, device="cuda") -> torch.Tensor:
-    """The rotation's table: 2^64 * theta^(-2i/D) / 2pi for i < D/2, rounded, modulo 2^64 (int64 bits).  A
-    position's angle in turns is the fraction position * turns / 2^64, exact to 2^-65 of the position."""
+    """The rotation's table: 2^64 * theta^(-2i/D) / 2pi for i < D/2, rounded (int64 bits).  A position's angle in
+    turns is the fraction position * turns / 2^64, exact to 2^-65 of the position (so the entries are computed to 60
+    digits: from 64-bit floats they are off by hundreds of their last place)."""
     if head_dim not in (64, 128) or not 1 <= theta < math.inf:
         raise ValueError(f"rope_turns: theta {theta} (at least 1), head_dim {head_dim} (64 or 128)")
-    vals = [round(theta ** (-2.0 * i / head_dim) / (2 * math.pi) * 2**64) % 2**64 for i in range(head_dim // 2)]
-    return torch.tensor([v - 2**64 if v >= 2**63 else v for v in vals], dtype=torch.int64, device=device)
+    vals = []
+    with decimal.localcontext(decimal.Context(prec=60, rounding=decimal.ROUND_HALF_EVEN)):
+        x, step = 2**63 / _PI, decimal.Decimal(float(theta)) ** (decimal.Decimal(-2) / head_dim)
+        for _ in range(head_dim // 2):
+            vals.append(int(x.to_integral_value()))
+            x *= step
+    return torch.tensor(vals, dtype=torch.int64, device=device)      # at most 2^64 / 2pi < 2^63
 
 
 def paged_qk_norm_rope_kv(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor, positions: torch.Tensor,

@@ -1,6 +1,7 @@
 """Refusals and host-side parts of the paged 8-bit serving operators (no GPU: every check comes before a launch)."""
 
 import math
+from fractions import Fraction
 
 import numpy as np
 import paged_oracle as oracle
@@ -49,6 +50,19 @@ def test_rope_turns(d, theta):
     # float64 power (the exponent's rounding counts ln(theta) < 14 times) and division: under 2^-48 relative; the
     # table's own rounding to whole 2^-64: half of one
     assert np.all(np.abs(got - want) <= want * 2.0 ** -48 + 2.0 ** -65)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("theta", [1, 1.0, 2.0, 1e4, 5e5, 1e6, 1234567.891, 1e300])
+def test_rope_turns_to_half_a_unit(d, theta):
+    """An entry t stands for the angle x = theta^(-2i/D) = 2 pi t / 2^64.  x^(D/2) = theta^-i is rational, so that
+    t - 1/2 <= 2^64 x / 2 pi <= t + 1/2 is decided in whole numbers, between two fractions of which one is below pi."""
+    scale = 10**40
+    below = Fraction(31415926535897932384626433832795028841971, scale)
+    for i, t in enumerate(ops.rope_turns(theta, d, device="cpu").numpy().view(np.uint64).tolist()):
+        want = Fraction(theta) ** -i
+        lo, hi = max(Fraction(2 * t - 1, 2), 0), Fraction(2 * t + 1, 2)
+        assert (lo * 2 * below / 2**64) ** (d // 2) <= want <= (hi * 2 * (below + Fraction(1, scale)) / 2**64) ** (d // 2), i
 
 
 @pytest.mark.parametrize("theta,d", [(0.0, 128), (-1.0, 128), (1e6, 96), (math.nan, 128), (math.inf, 128), (1e-300, 128)])
