@@ -387,7 +387,9 @@ sample_kernel(const bf16_t* __restrict__ logits, long long ld, int V, int turns,
     }
     keep = max(1, min(keep, n));
   }
-  if (mp > 0.0) {
+  if (mp > 1.0) {
+    keep = 1;                                    // no weight reaches it, the largest neither
+  } else if (mp > 0.0) {
     // tokens of a weight of at least min_p: weights fall along the bins, so look at every 1024th, then every 64th of
     // those, then each
     auto heavy = [&](int bin) { return bin <= first || weight(bin) >= mp; };

@@ -27,7 +27,8 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tenso
     temperature fp32 (1; at or below 0: the first maximum), top_k int32 (at or below 0: off), top_p fp32 (from 1:
     off), min_p fp32.  In the order of larger logits (equal ones: lower index), with weights exp((l - max) / T):
     the first top_k, of these the smallest prefix that has top_p of their weight, of these the ones of at least min_p
-    times the largest weight; the answer is the first whose running sum of weights exceeds uniform times their sum.
+    times the largest weight (the first stays in any case, alone where min_p is above 1); the answer is the first whose
+    running sum of weights exceeds uniform times their sum.
     -inf is a masked token; a row of nothing else gives -1 (probability 0).  A NaN counts as the maximum, as in
     ``decode_tail`` (probability NaN).  ``work`` from ``sample_workspace``."""
     if logits.dim() != 2:

@@ -238,3 +238,16 @@ def test_captured(ops):
             torch.cuda.synchronize()
         want, wp = ops.sample(x, u, t)
         assert torch.equal(tokens, want) and torch.equal(probs, wp)
+
+
+@pytest.mark.parametrize("mp", [1.0, 1.0000001, 1.5, math.inf])
+def test_min_p_above_one_keeps_the_first(ops, mp):
+    """No weight reaches a min_p above 1, not the maximum's either: of tied maxima the first is left."""
+    x = logits_of(3, 5000, 3)
+    x[0, [40, 700, 4999]] = 99.0
+    x[1] = 0.5
+    for t in (0.5, math.inf):
+        tokens, probs = check(ops, x, [0.9] * 3, t=[t] * 3, mp=[mp] * 3)
+        if mp > 1:
+            assert tokens.tolist() == [40, 0, int(x[2].argmax())] and probs.tolist() == [1.0] * 3
+    check(ops, x, [0.9] * 3, k=[2, 10, 2], p=[0.5, 0.9, 1.0], mp=[mp] * 3)
