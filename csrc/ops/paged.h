@@ -44,6 +44,11 @@ __device__ __forceinline__ int scale_exp(float amax) {
   const int e = x - 9 + ((u & 0x7fffffu) > 0x600000u);  // f > 0.875
   return min(max(e, EMIN), EMAX);
 }
+// a scale as the append makes them: a power of two, 2^EMIN to 2^EMAX
+__device__ __forceinline__ bool is_scale(float s) {
+  const uint32_t u = __float_as_uint(s);
+  return (u & 0x7fffffu) == 0 && u - ((uint32_t)(EMIN + 127) << 23) <= (uint32_t)(EMAX - EMIN) << 23;
+}
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // inclusive sum over the workgroup's NT threads (a multiple of 64); red: NT / 64 entries of shared memory.

@@ -92,6 +92,14 @@ __device__ __forceinline__ float2 get2(const float* at) {
   return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
+// The widening takes a scale's exponent only.  A page with a scale that is no power of two (or outside the append's range)
+// reads as NaN in K: rows that see it give NaN, not values that are up to twice too small.
+__device__ __forceinline__ void check_scales(float& ks, float& vs) {
+  const bool good = is_scale(ks) && is_scale(vs);
+  ks = good ? ks : __uint_as_float(0x7fc00000u);
+  vs = good ? vs : 1.f;
+}
+
 // a row's four values of head dimension d .. d+3; a row that saw no key (l = 0) gives zeros
 __device__ __forceinline__ void store_row(bf16_t* out, f32x4_t o, float l, int row, int tok0, int G, int Hq, int hk, int D,
                                           int d) {
@@ -279,7 +287,6 @@ __device__ __forceinline__ void short_part(const Call& c, const Work& k, int upt
   uint4 kr[4][KU], vr[DT];
   struct Page {
     size_t ph;
-    float ks, vs;
     bool bad;                                     // not a page of the cache: its keys count as masked
   };
   auto page_at = [&](int turn) {
@@ -291,8 +298,6 @@ __device__ __forceinline__ void short_part(const Call& c, const Work& k, int upt
     }
     const int id = __builtin_amdgcn_readlane(ids, turn & 63);
     Page x;
-    x.ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), turn & 63));
-    x.vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vss), turn & 63));
     x.bad = id < 0 || id >= pages;
     x.ph = (size_t)(x.bad ? 0 : id) * Hkv + hk;
     return x;
@@ -318,6 +323,9 @@ __device__ __forceinline__ void short_part(const Call& c, const Work& k, int upt
     load_v(cur.ph);
   }
   for (int turn = 0; turn < turns; ++turn) {
+    if ((turn & 63) == 0) check_scales(kss, vss);   // not where they are loaded: K and V need not wait for them
+    const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), turn & 63));
+    const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vss), turn & 63));
     f32x4_t s[4];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
@@ -325,8 +333,8 @@ __device__ __forceinline__ void short_part(const Call& c, const Work& k, int upt
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
         const uint4 c = kr[tt][u];
-        s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.x, c.y, cur.ks), qf[u][0], s[tt], 0, 0, 0);
-        s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.z, c.w, cur.ks), qf[u][1], s[tt], 0, 0, 0);
+        s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.x, c.y, ks), qf[u][0], s[tt], 0, 0, 0);
+        s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.z, c.w, ks), qf[u][1], s[tt], 0, 0, 0);
       }
     }
     if (turn + 1 < turns) {
@@ -367,7 +375,6 @@ __device__ __forceinline__ void short_part(const Call& c, const Work& k, int upt
         pf[h][j] = (__bf16)e;
       }
     if (live < PAGE) {                            // slots never written may hold any code, NaN too
-      if (cur.bad) cur.vs = 1.f;                  // page 0's, which may never have been written either
       const uint32_t m0 = live_bytes(16 * a, live), m1 = live_bytes(16 * a + 4, live), m2 = live_bytes(16 * a + 8, live),
                      m3 = live_bytes(16 * a + 12, live);
 #pragma unroll
@@ -376,8 +383,8 @@ __device__ __forceinline__ void short_part(const Call& c, const Work& k, int upt
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
       const uint4 c = vr[i];
-      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.x, c.y, cur.vs), pf[0], o[i], 0, 0, 0);
-      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.z, c.w, cur.vs), pf[1], o[i], 0, 0, 0);
+      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.x, c.y, vs), pf[0], o[i], 0, 0, 0);
+      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(c.z, c.w, vs), pf[1], o[i], 0, 0, 0);
     }
     if (turn + 1 < turns) load_v(next.ph);
     cur = next;
@@ -574,6 +581,7 @@ __device__ __forceinline__ void long_part(const Call& c, const Work& k, unsigned
       vss = vscale[x];
       // arrived: a wait here, every 64 pages, not behind the branch, where it would be for the codes on their way too
       asm volatile("" : "+v"(ids), "+v"(kss), "+v"(vss));
+      check_scales(kss, vss);
     }
     const int id = __builtin_amdgcn_readlane(ids, at);
     ks[z] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kss), at));
@@ -593,7 +601,6 @@ __device__ __forceinline__ void long_part(const Call& c, const Work& k, unsigned
       const int dim = t / (PAGE / 16), qk = t % (PAGE / 16), live = bad[z] ? 0 : L - p * PAGE;
       uint4& v = vr[z];
       if (live < PAGE) {                               // slots never written may hold any code, NaN too
-        if (bad[z]) vs[z] = 1.f;                       // page 0's, which may never have been written either
         v.x &= live_bytes(16 * qk, live);
         v.y &= live_bytes(16 * qk + 4, live);
         v.z &= live_bytes(16 * qk + 8, live);

@@ -165,7 +165,8 @@ class PagePool:
 
 class PagedKV(NamedTuple):
     """One layer's K and V: codes k [pages, Hkv, 64, D], v [pages, Hkv, D, 64] (torch.float8_e4m3fn), scales
-    k_scale, v_scale [pages, Hkv] fp32 (powers of two); a value is its code times its page's scale."""
+    k_scale, v_scale [pages, Hkv] fp32; a value is its code times its page's scale.  Scales are powers of two from
+    2^-110 to 2^119: a query that sees a page with any other gives NaN."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor

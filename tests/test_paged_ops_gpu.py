@@ -716,3 +716,53 @@ def test_plan_of_as_many_rows_as_there_are_indices(ops):
     assert torch.equal(plan.slots[:75], small.slots) and torch.equal(plan.positions[:75], small.positions)
     for t, v in ((plan.slots, -1), (plan.positions, 0)):
         assert int(t[75:].amin()) == v and int(t[75:].amax()) == v
+
+
+@pytest.mark.parametrize("new", [1, 50, 300])
+def test_attention_scales_that_are_no_powers_of_two(ops, new):
+    """Rows that see a page with such a scale (of K or of V, in their head) give NaN, all others what they give without."""
+    q, cache, table, cu, kv = attention_case(ops, [200, 300, 20], [new] * 3, 4, 2, 128)
+    args = (dev(table), dev(cu), dev(kv), 4, 2, 128, 0.1)
+    want = ops.paged_attention(q.cuda(), cache, *args)
+    last = (20 + new - 1) // PAGE                             # the third request's page that only its last rows see
+    above_one = float(np.nextafter(np.float32(1), np.float32(2)))
+    for bad in (1.5 * 2.0 ** -7, 1 / 448, above_one, -(2.0 ** -6), 0.0, math.inf, math.nan, 2.0 ** -111, 2.0 ** 120, 2.0 ** -149):
+        for side, b, h, page in (("k_scale", 0, 1, 1), ("v_scale", 1, 0, 0), ("v_scale", 2, 1, last)):
+            scale = getattr(cache, side).clone()
+            scale[table[b, page], h] = bad
+            got = ops.paged_attention(q.cuda(), cache._replace(**{side: scale}), *args).view(-1, 4, 128)
+            lost = torch.zeros(got.shape[:2], dtype=torch.bool)
+            lost[b * new:(b + 1) * new, 2 * h:2 * h + 2] = (torch.arange(new) + [200, 300, 20][b] >= page * PAGE)[:, None]
+            assert bool(lost.any()) and torch.equal(got.isnan().all(-1).cpu(), lost), (bad, side)
+            assert torch.equal(got[~lost.cuda()], want.view(-1, 4, 128)[~lost.cuda()]), (bad, side)
+    one = ops.paged_attention(q.cuda(), cache._replace(v_scale=torch.ones_like(cache.v_scale)), *args)
+    for e in (-110, 100):
+        far = cache._replace(v_scale=torch.full_like(cache.v_scale, 2.0 ** e))
+        assert torch.equal(ops.paged_attention(q.cuda(), far, *args), one * 2.0 ** e)
+
+
+@pytest.mark.parametrize("new,rows,hq,hkv", [(1, 520, 2, 1), (900, 1, 16, 8)])
+def test_attention_more_pages_than_lanes(ops, new, rows, hq, hkv):
+    """A wave's (a workgroup's) pages come in rounds of 64: requests of 300 shared pages, too many to be split far."""
+    r, d, pages = np.random.RandomState(0), 64, 300
+    cache = filled_cache(ops, pages, hkv, d, 1, garbage=False)
+    table, kv = r.randint(0, pages, (rows, 300)), r.randint(17000, 19201, rows)
+    q = (torch.randn(rows * new, hq, d) * 0.3).to(torch.bfloat16)
+    some = [0, rows // 3, rows - 1] if rows > 1 else [0]
+    for odd in (False, True):
+        if odd:                                       # past the first round, of one head
+            table[some[-1], 250] = pages
+            cache = ops.PagedKV(*(torch.cat([t.view(torch.uint8), t[:1].view(torch.uint8)]).view(t.dtype) for t in cache))
+            cache.k_scale[pages, 0] = 0.3
+        out = ops.paged_attention(q.cuda(), cache, dev(table), dev(np.arange(rows + 1) * new), dev(kv), hq, hkv, d, 0.125)
+        out = out.view(rows, new, hq, d)[some].cpu()
+        if odd:
+            assert out[-1, :, :hq // hkv].isnan().all()
+            assert out[:-1].isfinite().all() and out[:, :, hq // hkv:].isfinite().all()
+            continue
+        want, size = oracle.attention(q.view(rows, new, hq, d)[some].reshape(-1, hq, d), to_host(cache), table[some],
+                                      np.arange(len(some) + 1) * new, kv[some], hq, hkv, 0.125)
+        want, size = want.view(out.shape), size.view(out.shape)
+        # as in check_attention
+        tol = size * (2.0 ** -8 + 2.0 ** -9) + want.abs() * 2.0 ** -8 + 2.0 ** -100
+        assert torch.all((out.double() - want).abs() <= tol)
