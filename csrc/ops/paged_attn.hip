@@ -53,10 +53,13 @@ constexpr int short_rows(long long rows) {
   return rows <= FEW_ROWS ? FEW_ROWS : rows < MANY_ROWS ? 64 : 32;
 }
 
-// A call aims at as many workgroups as are resident (of the short ones two a CU, one beside long ones of D = 128; of the
-// long ones one), over all kv heads, and with that bounds the slots of the workspace: with t parts aimed at a kv head a
+// A call aims at as many workgroups as are resident (of the short ones two a CU, one beside long ones; of the long ones
+// one), over all kv heads, and with that bounds the slots of the workspace: with t parts aimed at a kv head a
 // split tile of np pages gets at most np / chunk + 1 <= 2 np / chunk parts, which add up to at most 2 t.
 constexpr int MAX_CUS = 256, MAX_HKV = 256;
+// (Beside long ones there is LDS for one, also with D = 64.  Aiming at two, 16 decoding requests of 4096 keys beside a
+// chunk of 1000, 8 / 8 heads of 64: 49 us instead of 42; 20 of 30 to 8000 beside 512, 32 / 4 heads: 25.3 and 23.)
+constexpr int short_resident(bool longs) { return longs ? 1 : 2; }
 constexpr int SHORT_SLOTS = 2 * 2 * MAX_CUS, LONG_SLOTS = 2 * MAX_CUS;
 
 // 8 codes -> 8 bf16, times 2^e
@@ -836,6 +839,15 @@ long long mivgpu_paged_attention_work(int N, int Hq, int Hkv, long long* zeroed)
   return ZEROED + SHORT_FLOATS + ((long long)N * (Hq / Hkv) > FEW_ROWS ? LONG_FLOATS : 0);
 }
 
+// Short workgroups that a call counts on for each CU, and in *fit how many of the kernel's the current GPU's CUs hold
+int mivgpu_paged_attention_resident(int head_dim, int longs, int* fit) {
+  const void* both = head_dim == 64 ? (const void*)attn_both_kernel<64> : (const void*)attn_both_kernel<128>;
+  const void* alone = head_dim == 64 ? (const void*)attn_kernel<64> : (const void*)attn_kernel<128>;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(fit, longs ? both : alone, longs ? LNT : 64 * SWAVES, 0) != hipSuccess)
+    return -1;
+  return short_resident(longs != 0);
+}
+
 // max_new: the most new tokens of a request, or negative if not known
 int mivgpu_paged_attention(const void* q, const void* kc, const void* vc, const float* kscale, const float* vscale,
                            const int* table, const int* cu, const int* kv_lens, void* out, float* work, long long floats,
@@ -863,8 +875,8 @@ int mivgpu_paged_attention(const void* q, const void* kc, const void* vc, const 
   long long tiles = rows / TILE + some, each = (long long)N * ((G + TILE - 1) / TILE);
   if (tiles > each) tiles = each;          // a token adds no more tiles than its own rows fill
   if (longs && tiles > some * (upto / TILE)) tiles = some * (upto / TILE);
-  // beside long ones short workgroups have eight waves, one a CU (two with D = 64), alone four, two a CU
-  const int waves = longs ? LWAVES : SWAVES, resident = (longs && head_dim == 128 ? 1 : 2) * all_cus();
+  // beside long ones short workgroups have eight waves, alone four
+  const int waves = longs ? LWAVES : SWAVES, resident = short_resident(longs) * all_cus();
   const int target = resident / Hkv > 1 ? resident / Hkv : 1;
   const long long few = rows / (upto + 1), ltiles = rows / LTILE + (few < some ? few : some);
   const long long parts = grid_of(tiles, target, waves) * Hkv, lparts = grid_of(ltiles, ltarget, LMIN_CHUNK) * Hkv;

@@ -1,5 +1,6 @@
 """The paged 8-bit serving operators on the GPU against plain 64-bit implementations (tests/paged_oracle.py)."""
 
+import ctypes
 import math
 
 import numpy as np
@@ -766,3 +767,12 @@ def test_attention_more_pages_than_lanes(ops, new, rows, hq, hkv):
         # as in check_attention
         tol = size * (2.0 ** -8 + 2.0 ** -9) + want.abs() * 2.0 ** -8 + 2.0 ** -100
         assert torch.all((out.double() - want).abs() <= tol)
+
+
+@pytest.mark.parametrize("longs", [0, 1])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_parts_are_resident(ops, d, longs):
+    """The parts that a call aims at have a place on the CUs: more would only add to the join."""
+    fit = ctypes.c_int(0)
+    aim = ops.lib().mivgpu_paged_attention_resident(d, longs, ctypes.byref(fit))
+    assert 1 <= aim <= fit.value
