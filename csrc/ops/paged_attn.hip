@@ -130,7 +130,8 @@ __device__ __forceinline__ int wave_scan(int v) {
 
 // Every wave scans all requests of more than `above` and at most `upto` rows by itself, 64 at once, in registers: no
 // barrier, and one round of loads.  Workgroup 0 takes the last part of all: in a prompt the tiles at the end have the
-// most keys, and the longest work should start first.  The caller sees to it that the sums fit 31 bits.
+// most keys, and the longest work should start first.  The caller sees to it that the sums fit 31 bits (and
+// no more is added to them).
 // Joining the parts of a short tile takes about 0.1 us a part, a page for each of its waves 1.5: at most sqrt(2 pages)
 // parts (one request of 131072 keys, 16 / 1 heads: 31 us against 53 with 256 parts; of 32768 20 against 23).
 template <int ROWS, int SMALLEST>
@@ -163,13 +164,13 @@ __device__ __forceinline__ Share find_share(const int* __restrict__ cu, const in
   const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
   // a tile's last part is mostly smaller than a chunk: leave a workgroup for each, so that all parts are resident at once
   const int goal = max(target - __builtin_amdgcn_readlane(wave_scan(some), 63), (target + 1) / 2);
-  const int chunk = max((total + goal - 1) / goal, SMALLEST);
+  const int chunk = max((total - 1) / goal + 1, SMALLEST);
   int all = 0;
 #pragma unroll
   for (int x = 0; x < PER; ++x) {
     if (64 * x >= B) break;
     const int most = ROWS == TILE ? min(MAX_PARTS, (int)__builtin_amdgcn_sqrtf(2.f * (float)np[x])) : MAX_PARTS;
-    np[x] = max(min((np[x] + chunk - 1) / chunk, most), 1);              // from here on: parts of a tile
+    np[x] = max(min((np[x] - 1) / chunk + 1, most), 1);                  // from here on: parts of a tile
     all += tiles[x] * np[x];
   }
   all = __builtin_amdgcn_readlane(wave_scan(all), 63);

@@ -776,3 +776,16 @@ def test_attention_parts_are_resident(ops, d, longs):
     fit = ctypes.c_int(0)
     aim = ops.lib().mivgpu_paged_attention_resident(d, longs, ctypes.byref(fit))
     assert 1 <= aim <= fit.value
+
+
+def test_attention_as_many_pages_as_there_are_indices(ops):
+    """64 tiles of 2^25 - 1 pages, one below 2^31 in all: none but a request's last is in the cache."""
+    W, n = 2**25 - 1, 64
+    cache = filled_cache(ops, 2, 1, 64, 0, garbage=False)
+    q = torch.randn(n, 16, 64, device="cuda").to(torch.bfloat16)
+    want = ops.paged_attention(q, cache, dev([[1]]), dev([0, n]), dev([PAGE]), 16, 1, 64, 0.125, max_new=1)   # the same kernel
+    table = torch.full((1, W), -1, dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    out = torch.full((n, 16 * 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    ops.paged_attention(q, cache, table, dev([0, n]), dev([W * PAGE]), 16, 1, 64, 0.125, max_new=1, out=out)
+    assert torch.equal(out, want)
