@@ -278,8 +278,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, table: torch.Tensor, cu_q: 
     pages, specs = _cache_specs(cache, name, n_q_heads, n_kv_heads, head_dim)
     if n_kv_heads > MAX_KV_HEADS:
         raise ValueError(f"{name}: {n_kv_heads} kv heads (at most {MAX_KV_HEADS})")
-    if q.dim() != 3 or not 0 < scale < math.inf:
-        raise ValueError(f"{name}: q must be [N, {n_q_heads}, {head_dim}], got {list(q.shape)}, and scale positive, got {scale}")
+    if q.dim() != 3 or not 2.0 ** -126 <= scale <= 2.0 ** 126:      # a normal fp32 number, times log2(e) too
+        raise ValueError(f"{name}: q must be [N, {n_q_heads}, {head_dim}], got {list(q.shape)}, and scale in "
+                         f"2^-126 .. 2^126, got {scale}")
     N = q.shape[0]
     B, W = table.shape if table.dim() == 2 else (0, 0)
     if not 0 < B <= MAX_ROWS or not 0 < W <= (2**31 - 1) // PAGE:

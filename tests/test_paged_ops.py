@@ -141,6 +141,19 @@ def test_attention_refuses(bad):
         ops.paged_attention(**attn_args(**bad))
 
 
+@pytest.mark.parametrize("scale", [0.0, -1.0, 1e-50, 2.0 ** -127, 2.0 ** 127, 1e39, math.inf, math.nan])
+def test_attention_refuses_scales_that_fp32_lacks(scale):
+    """As fp32 these are 0 or infinite: 0 times a masked score's -inf would be NaN."""
+    with pytest.raises(ValueError, match="paged_attention: q must be .* scale"):
+        ops.paged_attention(**attn_args(scale=scale))
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -126, 1e-30, 1, 1e30, 2.0 ** 126])
+def test_attention_takes_scales_that_fp32_has(scale):
+    with pytest.raises(ValueError, match="on one GPU"):
+        ops.paged_attention(**attn_args(scale=scale))
+
+
 @pytest.mark.parametrize("args", [(-1, 1, 4, 2, 128), (2**31, 1, 4, 2, 128), (1, 0, 4, 2, 128), (1, 1025, 4, 2, 128), (1, 1, 5, 2, 128),
                                   (1, 1, 4, 0, 128), (1, 1, 257, 257, 64), (1, 1, 4, 2, 96)])
 def test_attention_workspace_refuses(args):
