@@ -789,3 +789,103 @@ def test_attention_as_many_pages_as_there_are_indices(ops):
     out = torch.full((n, 16 * 64), 5.0, dtype=torch.bfloat16, device="cuda")
     ops.paged_attention(q, cache, table, dev([0, n]), dev([W * PAGE]), 16, 1, 64, 0.125, max_new=1, out=out)
     assert torch.equal(out, want)
+
+
+# ------------------------------------------------- closer looks at the same --
+@pytest.mark.parametrize("grow", [1, -1])
+@pytest.mark.parametrize("case", ["single", "a few each", "prompts", "chunk beside decode", "long chunk", "chunk beside a few, heads of 64"])
+def test_attention_scores_that_grow_along_the_pages(ops, case, grow):
+    """Keys of twice the size from page to page (or half), queries from 2^-6 to 2^6: maxima that move by less and by more
+    than a factor of 2^8 of the weights, scores in the thousands.  A query has one value that is not zero, so that its
+    scores are exact in fp32 and the bounds are those of check_attention."""
+    old, new, hq, hkv, d = ATTNS[case]
+    q, cache, table, cu, kv = attention_case(ops, old, new, hq, hkv, d)
+    r = np.random.RandomState(1)
+    for b in range(len(kv)):
+        for j in range(-(-int(kv[b]) // PAGE)):
+            cache.k_scale[table[b, j]] = 2.0 ** (-9 + (j if grow > 0 else -j) % 10)
+    one = torch.zeros(q.numel() // d, d, dtype=torch.bfloat16)
+    at, size = r.randint(0, d, len(one)), 2.0 ** r.randint(-6, 7, len(one)) * r.choice([-1, 1], len(one))
+    one[torch.arange(len(one)), torch.as_tensor(at)] = torch.as_tensor(size).to(torch.bfloat16)
+    check_attention(ops, one.view(q.shape), cache, table, cu, kv, hq, hkv, d, scale=1.0)
+
+
+@pytest.mark.parametrize("old,new,hq,hkv,d", [
+    ([500], [2048], 16, 16, 128), ([500], [2048], 32, 8, 128), ([2000], [512], 16, 16, 64), ([0], [1100], 16, 16, 64),
+    ([700, 2000, 64, 900], [700, 1, 3, 1], 16, 16, 64), ([0, 300, 4000], [1000, 900, 1], 8, 4, 128)])
+def test_attention_tiles_of_unlike_lengths(ops, old, new, hq, hkv, d):
+    """Prompts and chunks of some tiles a head, the last of several times the first one's pages, with CUs over."""
+    q, cache, table, cu, kv = attention_case(ops, old, new, hq, hkv, d, seed=4)
+    work = ops.paged_attention_workspace(len(q), len(old), hq, hkv, d)
+    a = check_attention(ops, q, cache, table, cu, kv, hq, hkv, d, work=work)
+    for _ in range(3):
+        out = torch.full_like(a, 5.0)
+        ops.paged_attention(q.cuda(), cache, dev(table), dev(cu), dev(kv), hq, hkv, d, 1 / math.sqrt(d), out=out, work=work)
+        assert torch.equal(out, a)
+
+
+def test_attention_leaves_every_counter_at_zero(ops):
+    work, zeroed = ops.paged_attention_workspace(1024, 64, 32, 1, 128), ctypes.c_longlong(0)
+    ops.lib().mivgpu_paged_attention_work(1024, 32, 1, ctypes.byref(zeroed))
+    assert zeroed.value > 1024
+    for name in ATTNS:
+        old, new, hq, hkv, d = ATTNS[name]
+        q, cache, table, cu, kv = attention_case(ops, old, new, hq, hkv, d)
+        ops.paged_attention(q.cuda(), cache, dev(table), dev(cu), dev(kv), hq, hkv, d, 0.1, work=work)
+        assert (work[:zeroed.value].view(torch.int32) == 0).all(), name
+
+
+APPEND_MENDS = {
+    "larger": lambda x: x.mul_(2.0 ** 9), "smaller": lambda x: x.mul_(2.0 ** -9), "far larger": lambda x: x.mul_(2.0 ** 40),
+    "zeros": lambda x: x.zero_(), "some zeros": lambda x: x[::3].zero_(), "huge V": lambda x: x[:, 6 * 128:].fill_(-3.3e38),
+    "NaN in K": lambda x: x[2:70:17, 4 * 128 + 5].fill_(math.nan), "inf in V": lambda x: x[1::9, 7 * 128 + 9].fill_(math.inf),
+    "NaN in q": lambda x: x[5, 128 + 3].fill_(math.nan),
+}
+
+
+@pytest.mark.parametrize("name", APPEND_MENDS, ids=list(APPEND_MENDS))
+def test_append_of_unusual_values_q_too(ops, name):
+    """q of every head whose inputs are finite, whatever stands in the others."""
+    old, new, seed, (hq, hkv, d), seen = [7, 100, 0], [3, 1, 75], 5, (4, 2, 128), []
+
+    def mend(x):
+        APPEND_MENDS[name](x)
+        seen.append(x.clone())
+    q_out, _ = check_append(ops, old, new, hq, hkv, d, mend=mend, seed=seed)
+    pos, g = layout(old, new, seed)[0], torch.Generator()
+    g.manual_seed(seed)                               # the norm's weights, as check_append draws them
+    torch.randn(len(pos), (hq + 2 * hkv) * d, generator=g), torch.rand((hq + 2 * hkv) * d, generator=g)
+    qw = (1 + 0.1 * torch.randn(d, generator=g)).to(torch.bfloat16)
+    x = seen[0][:, :hq * d].double().view(-1, hq, d)
+    q, size = oracle.norm_rope(x, qw.double(), pos, THETA, EPS)
+    fine = x.isfinite().all(-1)
+    got = q_out.cpu().double()
+    assert torch.all(((got - q).abs() <= q.abs() * 2.0 ** -8 + size * 2.0 ** -18)[fine])      # as in check_append
+    assert got[~fine].isnan().any(-1).all() and int(fine.sum()) >= len(pos) * hq - 1
+
+
+def test_steps_together_layer_by_layer(ops):
+    """As test_steps_together, with each layer's queries kept: both layers' attention is the oracle's."""
+    class Keep:
+        def __getattr__(self, name):
+            return getattr(ops, name)
+
+        def paged_attention(self, q, *args, **kw):
+            queries.append(q.clone())
+            return ops.paged_attention(q, *args, **kw)
+
+    s = server(ops, 200, 3)
+    for new in ([70, 0, 30], [1, 100, 1], [1, 1, 1], [0, 1, 66]):
+        s["x"].add_(0.125)
+        queries = []
+        plan = serve_step(Keep(), s, dev(new), 200)
+        n = sum(new)
+        assert len(queries) == 2
+        for q, cache, att in zip(queries, s["cache"], s["att"]):
+            c = to_host(cache)
+            for t in (c.k, c.v):
+                t.view(torch.uint8).copy_(torch.where((t.view(torch.uint8) & 0x7f) == 0x7f, 0, t.view(torch.uint8)))
+            o, size = oracle.attention(q.cpu(), c, host(s["pool"].table), host(plan.cu_q), host(plan.kv_lens), 8, 2, 1 / math.sqrt(128))
+            o, size = o.reshape(200, -1), size.reshape(200, -1)
+            tol = size * (2.0 ** -8 + 2.0 ** -9) + o.abs() * 2.0 ** -8 + 2.0 ** -100
+            assert torch.all((att.cpu().double() - o).abs()[:n] <= tol[:n])
