@@ -523,11 +523,13 @@ __device__ __forceinline__ void short_part(const Call& c, const Work& k, int upt
 // which neither bf16 nor the sums mind.
 // Measured on an 8192-token prompt, 32 / 8 heads: 514 us, 1070 TFLOP/s; with the stores before the barrier instead of
 // between the pages 525, a barrier a page 568, the buffers picked at run time 551.  The matrix units are busy half of
-// the time and the vector units the other half, at a clock of 1.9 to 2.1 GHz of the card's 2.4: hiding more latency
-// gains nothing (operands read three steps ahead 511; the next page's scores beside this one's exponentials in a wave
-// 528), less work does (without the stores and loads it would be 396).  Left out: the two waves of a SIMD half a page
-// apart, one's matrix instructions beside the other's exponentials, two barriers a page (653; 614 without the offset);
-// four waves of 64 rows, which halve the LDS reads, the next page's scores beside this one's exponentials (792).
+// the time and the vector units the other half, one after the other, at a clock of 1.9 to 2.1 GHz of the card's 2.4.
+// That is no limit of the card: in a probe, matrix instructions of one wave and vector ones of another on a SIMD do
+// overlap (0.242 and 0.237 ms alone, 0.305 together).  Nothing tried here made the loop do so: operands read three steps
+// ahead 511, the next page's scores beside this one's exponentials in a wave 528, the two waves of a SIMD half a page
+// apart, one's matrix instructions beside the other's exponentials, two barriers a page 653 (614 without the offset), four
+// waves of 64 rows, which halve the LDS reads, with the next page's scores beside this one's exponentials 792.  Less work
+// gains time: without the stores and loads it would be 396.
 template <int D>
 __device__ __forceinline__ int k_at(int row, int ch) { return row * D + ((ch ^ (row & (D / 8 - 1))) << 3); }
 __device__ __forceinline__ int v_at(int dim, int ch) { return dim * PAGE + ((ch ^ ((dim >> 1) & 7)) << 3); }

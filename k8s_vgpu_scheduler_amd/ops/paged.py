@@ -270,10 +270,11 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, table: torch.Tensor, cu_q: 
                     out: torch.Tensor | None = None, work: torch.Tensor | None = None) -> torch.Tensor:
     """Causal GQA attention of packed tokens over their requests' pages -> out [N, Hq*D] bf16.
 
-    q [N, Hq, D] bf16; request b owns rows cu_q[b] .. cu_q[b+1], the last of its kv_lens[b] positions; its pages are
-    table[b] (int32 [B, W], B <= 1024).  A row that sees no key (a request with kv_lens 0) gives zeros; rows behind
-    cu_q[B] are left as they are; keys on a page that the cache does not have count as masked.  ``max_new``: the most
-    new tokens of a request, if known (1 in a decode step, which is then faster for many requests).  ``work`` from ``paged_attention_workspace``."""
+    q [N, Hq, D] bf16; request b owns rows cu_q[b] .. cu_q[b+1], the last of its kv_lens[b] positions (at most 64 W); its
+    pages are table[b] (int32 [B, W], B <= 1024).  A row that sees no key (a request with kv_lens 0) gives zeros; rows
+    behind cu_q[B] are left as they are; keys on a page that the cache does not have count as masked.  ``max_new``: the
+    most new tokens of a request, if known (1 in a decode step, which is then faster for many requests).  ``work`` from
+    ``paged_attention_workspace``."""
     name = "paged_attention"
     pages, specs = _cache_specs(cache, name, n_q_heads, n_kv_heads, head_dim)
     if n_kv_heads > MAX_KV_HEADS:
